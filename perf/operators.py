@@ -211,7 +211,7 @@ def run(s):
     op, x = case["op"], s["x"]
     if op == "quantise":
         return ops.mx4_quantize(x).dequantize(torch.bfloat16)
-    w = ops.Mx4Matrix(s["codes"], s["tiles"])
+    w = ops.Mx4Matrix(s["codes"], s["tiles"], settled=True)          # a loaded model's weight: nothing writes it any more
     if op == "linear":
         return ops.linear(x, w, out_dtype=torch.bfloat16 if case["out"] == "bf16" else torch.float32)
     if op == "gated":
