@@ -44,6 +44,8 @@ LIBRARIES = {
     "tc2": (["gemm_tc2.cu"], []),
     "group": (["gemm_group.cu"], []),
     "stream": (["gemv_stream.cu"], []),
+    "mx4": (["mx4.cu"], []),
+    "mx4_tc": (["gemm_mx4.cu"], []),
     "attn_tc": (["attention_tc.cu"], []),
     "host": (["host_runtime.cpp"], []),
 }

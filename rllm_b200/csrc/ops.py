@@ -1473,7 +1473,7 @@ def check_device_errors(device="cuda:0") -> None:
 
 
 _WAIT_LIBRARIES = {"tc": "rllm_tc", "tc2": "rllm_tc2", "stream": "rllm_stream", "attn_tc": "rllm_attn_tc",
-                   "group": "rllm_gemm_group"}
+                   "group": "rllm_gemm_group", "mx4_tc": "rllm_gemm_mx4"}
 
 
 def set_wait_cycles(cycles: int = 0, libraries=None) -> None:
@@ -1830,7 +1830,12 @@ def linear(a, w, out=None, out_dtype=None, accumulate=False, stream=None, follow
     float32 operands always take the CUDA-core products of gemm_f32.cu (the true 32-bit path).
     bfloat16 operands: up to 64 rows take the weight-streaming tensor-core kernel, more rows the
     library product; shapes neither can take (a row length that is not a multiple of 8
-    elements) take the plain product with the same operand types."""
+    elements) take the plain product with the same operand types.
+    A weight of microscaled 4-bit numbers (Mx4Matrix): the rows become such numbers too (mx4_linear)."""
+    if isinstance(w, Mx4Matrix):
+        if isinstance(a, NormedRows) or then_norm is not None:
+            raise KernelError("linear: a deferred norm does not go with a 4-bit weight (ask defers_norm first)")
+        return mx4_linear(a, w, out, out_dtype, accumulate)
     m, k = a.shape
     n = w.shape[0]
     if out is None:
@@ -1919,7 +1924,12 @@ def gate_up_swiglu(h, w_gate_up, out, glu=None):
     float32 and odd shapes: a product followed by the activation kernel.
     glu = (limit, alpha, shift): another gated form, g sigmoid(alpha g) (u + shift) with g = min(gate,
     limit), u = clamp(up, -limit, limit); the tcgen05 kernels take it in their epilogue, fewer rows and
-    the other shapes a product followed by the activation kernel."""
+    the other shapes a product followed by the activation kernel.
+    w_gate_up may be a stack [2, F, k] of microscaled 4-bit numbers (Mx4Matrix): mx4_gated."""
+    if isinstance(w_gate_up, Mx4Matrix):
+        if isinstance(h, NormedRows):
+            raise KernelError("gate_up_swiglu: a deferred norm does not go with a 4-bit weight")
+        return mx4_gated(h, w_gate_up, out, glu)
     m = h.shape[0]
     F = out.shape[1]
     rows = h.xw if isinstance(h, NormedRows) else h
@@ -1939,6 +1949,249 @@ def gate_up_swiglu(h, w_gate_up, out, glu=None):
         return _gemm_gated(h, w_gate_up, out)            # tcgen05, activation in the epilogue
     gu = linear(h, w_gate_up, out_dtype=torch.float32)     # same rounding points as the fused kernels
     return silu_mul(gu, out)
+
+
+# ------------------------------------------------------------------ microscaled 4-bit numbers (mx4.cu, gemm_mx4.cu)
+
+MX4_BLOCK = 32                 # neighbouring entries of a row that share a scale
+MX4_MAX_EXPERTS = 1024
+
+
+class Mx4Matrix:
+    """A matrix [n, k], or a stack of them [..., n, k], of microscaled 4-bit numbers (MXFP4): `codes` uint8 [..., n, k / 2], two
+    entries to a byte, the even one in the low half; `scales` uint8 [..., ceil(n / 128), 2 ceil(k / 256), 32, 4, 4], the scale of
+    row r and block b (32 entries) at [r // 128, b // 4, r % 32, r // 32 % 4, b % 4], zeros behind the last block of a row.
+    An entry is e2m1(code) * 2^(scale - 127); scale 255: not a number.  Made by `mx4_quantize`, by `from_blocks`, or from the two tensors.
+
+    `linear` and `gate_up_swiglu` take one in place of a weight.  settled: the caller knows that no kernel that writes codes or scales is still
+    in flight (the weights of a loaded model); products may then read them before the kernels launched before have ended."""
+    __slots__ = ("codes", "scales", "settled")
+
+    def __init__(self, codes, scales, settled=False):
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 2 or scales.dim() != codes.dim() + 3:
+            raise KernelError("Mx4Matrix: codes are uint8 [..., n, k / 2], scales uint8 [..., n / 128, k / 128, 32, 4, 4]")
+        n, k = codes.shape[-2], 2 * codes.shape[-1]
+        if k % MX4_BLOCK or k == 0:
+            raise KernelError(f"Mx4Matrix: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
+        if scales.shape != codes.shape[:-2] + mx4_scale_shape(n, k) or scales.device != codes.device:
+            raise KernelError(f"Mx4Matrix: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)}")
+        if not codes.is_contiguous() or not scales.is_contiguous() or (codes.data_ptr() | scales.data_ptr()) % 16:
+            raise KernelError("Mx4Matrix: codes and scales must be contiguous and begin at a multiple of 16 bytes")
+        self.codes, self.scales, self.settled = codes, scales, settled
+
+    @classmethod
+    def from_blocks(cls, codes, scales, settled=False):
+        """From scales in rows, uint8 [..., n, k / 32], as a checkpoint holds them."""
+        n, g = scales.shape[-2:]
+        lead = tuple(scales.shape[:-2])
+        shape = mx4_scale_shape(n, MX4_BLOCK * g)
+        t = scales.new_zeros(lead + (shape[0] * 128, shape[1] * 4))
+        t[..., :n, :g] = scales
+        t = t.view(lead + (shape[0], 4, 32, shape[1], 4))
+        i = len(lead)
+        return cls(codes, t.permute(*range(i), i, i + 3, i + 2, i + 1, i + 4).contiguous(), settled)
+
+    def block_scales(self):
+        """The scales in rows, uint8 [..., n, k / 32]."""
+        *lead, n, k = self.shape
+        s, i = self.scales, len(lead)
+        s = s.permute(*range(i), i, i + 3, i + 2, i + 1, i + 4).reshape(*lead, s.shape[i] * 128, s.shape[i + 1] * 4)
+        return s[..., :n, :k // MX4_BLOCK].contiguous()
+
+    def dequantize(self, dtype=torch.float32):
+        """The values [..., n, k] (exact in float32 and in bfloat16)."""
+        _need_cuda(self.codes, self.scales)
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        n, k = self.shape[-2:]
+        if out.numel():
+            _mx4_current(self)
+            _check(_lib("mx4").rllm_mx4_dequantize(_ptr(self.codes), _ptr(self.scales), c_longlong(self.matrices), c_int(n), c_int(k),
+                                                   _ptr(out), c_int(_code(out)), _stream()), "mx4_dequantize")
+        return out
+
+    @property
+    def shape(self):
+        return self.codes.shape[:-1] + (2 * self.codes.shape[-1],)
+
+    @property
+    def matrices(self):
+        m = 1
+        for s in self.codes.shape[:-2]:
+            m *= s
+        return m
+
+    @property
+    def dtype(self):
+        return self.codes.dtype
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def is_cuda(self):
+        return self.codes.is_cuda
+
+    def tensors(self):
+        return self.codes, self.scales
+
+
+def mx4_scale_shape(n: int, k: int) -> tuple:
+    """Shape of the scales of a matrix [n, k] (see Mx4Matrix)."""
+    return (-(-n // 128), 2 * -(-k // 256), 32, 4, 4)
+
+
+def _mx4_current(*ts):
+    """The launchers take the current device's stream: every operand has to be there."""
+    for t in ts:
+        if t is not None and t.device.index not in (None, _current_device()):
+            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{_current_device()}")
+
+
+def _mx4_rows(x, who):
+    if x.dim() != 2 or x.stride(1) != 1:
+        raise KernelError(f"{who}: rows [m, k] with neighbouring entries side by side, got {tuple(x.shape)} with strides {x.stride()}")
+    if x.shape[1] % MX4_BLOCK or x.shape[1] == 0:
+        raise KernelError(f"{who}: rows of {x.shape[1]} entries are not whole blocks of {MX4_BLOCK}")
+    return x
+
+
+def _mx4_quantize(x, codes, scales, pad, offsets=None, place=None, experts=0, top_k=0):
+    rows = codes.shape[0]
+    _check(_lib("mx4").rllm_mx4_quantize(_ptr(x), c_int(_code(x)), c_longlong(x.stride(0)), c_int(rows), c_int(x.shape[1]), _ptr(codes),
+                                         _ptr(scales), c_int(pad), _ptr(offsets), _ptr(place), c_int(experts), c_int(top_k), _stream()),
+           "mx4_quantize")
+
+
+def mx4_quantize(x):
+    """x [..., n, k] float32 or bfloat16 (k a multiple of 32; a matrix may have any row stride) as an Mx4Matrix.  A block's scale is 2^(floor(log2 of
+    its largest magnitude) - 2), at least 2^-127; entries are rounded to the nearest code, ties to the even one, at most 6 scales; a block
+    with an infinity or a NaN becomes NaN.  See mx4.cuh."""
+    _need_cuda(x)
+    _mx4_current(x)
+    if x.dim() > 2:
+        _need_contig(x=x)
+    _mx4_rows(x if x.dim() <= 2 else x.view(-1, x.shape[-1]), "mx4_quantize")
+    *lead, n, k = x.shape
+    codes = torch.empty((*lead, n, k // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(tuple(lead) + mx4_scale_shape(n, k), dtype=torch.uint8, device=x.device)
+    if x.numel():
+        if x.dim() == 2:
+            _mx4_quantize(x, codes, scales, 1)
+        elif n % 128 == 0:                             # the stack is one matrix as far as rows and scale rows go
+            _mx4_quantize(x.view(-1, k), codes.view(-1, k // 2), scales, 1)
+        else:                                          # every matrix has scale rows of its own
+            c, s = codes.view(-1, n, k // 2), scales.view(-1, *scales.shape[-5:])
+            for i, m in enumerate(x.view(-1, n, k)):
+                _mx4_quantize(m, c[i], s[i], 1)
+    return Mx4Matrix(codes, scales)
+
+
+def _mx4_operand(x, who):
+    """Rows as a product's first operand: (codes, scales); nothing behind the last row is written."""
+    _mx4_rows(x, who)
+    m, k = x.shape
+    codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(mx4_scale_shape(m, k), dtype=torch.uint8, device=x.device)
+    _mx4_quantize(x, codes, scales, 0)
+    return codes, scales
+
+
+def _gemm_mx4(codes, scales, w, out, n, epilogue, glu=None, offsets=None, experts=1):
+    limit, alpha, shift = glu or (0.0, 1.0, 0.0)
+    st = _lib("mx4_tc").rllm_gemm_mx4(
+        _ptr(codes), _ptr(scales), _ptr(w.codes), _ptr(w.scales), _ptr(out), c_int(_code(out)), c_longlong(out.stride(0)), _ptr(offsets),
+        c_int(experts), c_int(codes.shape[0]), c_int(n), c_int(2 * codes.shape[1]), c_int(epilogue), c_int(1 if w.settled else 0),
+        c_float(limit), c_float(alpha), c_float(shift), _ptr(error_word(codes.device)), _stream())
+    if st >= 30000:
+        raise KernelError(f"gemm_mx4: tensor map encoding failed (CUresult {st - 30000})")
+    _check(st, "gemm_mx4")
+    return out
+
+
+def _mx4_product(x, w, out, n, lead, who):
+    """Checks that the products have in common: x [m, k], w a stack `lead` of [n, k], out [m, n]."""
+    _need_cuda(x, w, out)
+    _mx4_current(x, w, out)
+    _mx4_rows(x, who)
+    if tuple(w.shape) != tuple(lead) + (n, x.shape[1]):
+        raise KernelError(f"{who}: a weight {tuple(w.shape)} where {tuple(lead) + (n, x.shape[1])} is needed")
+    if out.dim() != 2 or out.shape[1] != n or (n > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < n):
+        raise KernelError(f"{who}: an output {tuple(out.shape)} with strides {out.stride()} for {n} columns")
+
+
+def mx4_linear(x, w, out=None, out_dtype=None, accumulate=False):
+    """out [m, n] (+)= Q(x) W^T: the rows x [m, k] (float32 or bfloat16) become 4-bit numbers as by `mx4_quantize`, w [n, k] is an
+    Mx4Matrix; products of 4-bit numbers with float32 sums.  accumulate: `out` is float32 and the product is added to it."""
+    m, n = x.shape[0], w.shape[0]
+    if out is None:
+        if accumulate:
+            raise KernelError("mx4_linear: accumulate needs an output to add to")
+        out = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+    _mx4_product(x, w, out, n, (), "mx4_linear")
+    if out.shape[0] != m:
+        raise KernelError(f"mx4_linear: an output of {out.shape[0]} rows for {m}")
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError("accumulating product needs a float32 output")
+    if m and n:
+        _gemm_mx4(*_mx4_operand(x, "mx4_linear"), w, out, n, EPI_ACCUM if accumulate else EPI_STORE)
+    return out
+
+
+def mx4_gated(h, w, out, glu=None):
+    """out [m, F] = glu(Q(h) Wg^T, Q(h) Wu^T), w the stack [2, F, k] of gate and up; glu = (limit, alpha, shift) as for
+    gate_up_swiglu (None: SwiGLU)."""
+    m, F = out.shape
+    _mx4_product(h, w, out, F, (2,), "mx4_gated")
+    if h.shape[0] != m:
+        raise KernelError(f"mx4_gated: an output of {m} rows for {h.shape[0]}")
+    if m and F:
+        _gemm_mx4(*_mx4_operand(h, "mx4_gated"), w, out, F, EPI_SWIGLU, glu)
+    return out
+
+
+def _mx4_sorted(x, rows, offsets, place, experts, who):
+    """The sorted rows of routed experts as an operand: x the tokens' rows with `place`, or the sorted rows themselves."""
+    k = x.shape[1]
+    if not 0 < experts <= MX4_MAX_EXPERTS:
+        raise KernelError(f"{who}: {experts} experts (1 to {MX4_MAX_EXPERTS})")
+    for name, t, size in (("offsets", offsets, experts + 1), ("place", place, rows)):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != size):
+            raise KernelError(f"{who}: {name} is int32 [{size}]")
+    _need_cuda(offsets, place)
+    _mx4_current(offsets, place)
+    codes = torch.empty((rows, k // 2), dtype=torch.uint8, device=x.device)
+    # every expert's rows begin a block of 128 scale rows
+    scales = torch.empty((-(-rows // 128) + experts,) + mx4_scale_shape(1, k)[1:], dtype=torch.uint8, device=x.device)
+    _mx4_quantize(x, codes, scales, 0, offsets, place, experts, rows // x.shape[0] if place is not None else 0)
+    return codes, scales
+
+
+def mx4_experts_up(h, w, offsets, place, act, glu=None):
+    """The gated product of routed experts: act[place[p]] = glu(Q(h[p // top_k]) Wg[e]^T, Q(h[p // top_k]) Wu[e]^T) for the pairs p of
+    h [n, d] with their experts e, sorted by `moe_sort` (offsets [E + 1], place [n * top_k]); w [E, 2, F, d] as an Mx4Matrix, act
+    [n * top_k, F].  Two launches, whatever the experts' counts; no host involvement."""
+    pairs, F = act.shape
+    if len(w.shape) != 4 or h.dim() != 2 or (h.shape[0] and pairs % h.shape[0]) or (pairs and not h.shape[0]):
+        raise KernelError(f"mx4_experts_up: {pairs} pairs of {tuple(h.shape)} rows, weights {tuple(w.shape)}")
+    E = w.shape[0]
+    _mx4_product(h, w, act, F, (E, 2), "mx4_experts_up")
+    if pairs and F:
+        _gemm_mx4(*_mx4_sorted(h, pairs, offsets, place, E, "mx4_experts_up"), w, act, F, EPI_SWIGLU, glu, offsets, E)
+    return act
+
+
+def mx4_experts_down(act, w, offsets, y):
+    """The experts' second product: y[r] = Q(act[r]) W[e]^T for the sorted rows r of expert e (offsets [E + 1]); w [E, n, k] as an
+    Mx4Matrix, y [rows, n] float32 or bfloat16.  `moe_combine` adds a token's rows up with the router's weights."""
+    rows, n = y.shape
+    if len(w.shape) != 3 or act.dim() != 2 or act.shape[0] != rows:
+        raise KernelError(f"mx4_experts_down: {tuple(act.shape)} rows, weights {tuple(w.shape)}, output {tuple(y.shape)}")
+    E = w.shape[0]
+    _mx4_product(act, w, y, n, (E,), "mx4_experts_down")
+    if rows and n:
+        _gemm_mx4(*_mx4_sorted(act, rows, offsets, None, E, "mx4_experts_down"), w, y, n, EPI_STORE, None, offsets, E)
+    return y
 
 
 FLASH_HEAD_DIMS = (64, 128)

@@ -1,0 +1,48 @@
+"""What of the microscaled 4-bit numbers needs no GPU: the layout of the scales, and what is refused."""
+import pytest
+import torch
+
+import plain_mx4 as plain
+from rllm_b200.csrc import ops
+
+
+@pytest.mark.parametrize("lead,n,k", [((), 1, 32), ((), 130, 288), ((2,), 128, 256), ((3, 2), 5, 544)])
+def test_scale_layout(lead, n, k):
+    g = torch.Generator().manual_seed(1)
+    codes = torch.randint(0, 256, (*lead, n, k // 2), generator=g).to(torch.uint8)
+    scales = torch.randint(0, 256, (*lead, n, k // 32), generator=g).to(torch.uint8)
+    m = ops.Mx4Matrix.from_blocks(codes, scales)
+    assert m.shape == (*lead, n, k) and m.scales.shape == (*lead, *ops.mx4_scale_shape(n, k))
+    assert torch.equal(m.block_scales(), scales)
+    tiles, rows = m.scales.view(-1, *m.scales.shape[-5:]), scales.view(-1, n, k // 32)
+    for i in range(rows.shape[0]):
+        for r in range(0, n, 7):
+            for b in range(k // 32):
+                assert tiles[i, r // 128, b // 4, r % 32, r // 32 % 4, b % 4] == rows[i, r, b]
+    assert int(m.scales.long().sum()) == int(scales.long().sum())          # zeros elsewhere
+
+
+def test_refusals():
+    codes = torch.zeros(4, 32, dtype=torch.uint8)
+    scales = torch.zeros(ops.mx4_scale_shape(4, 64), dtype=torch.uint8)
+    ops.Mx4Matrix(codes, scales)
+    for c, s in ((codes.int(), scales), (codes, scales.float()), (codes[0], scales), (codes, scales[0]), (codes[:, :24], scales),
+                 (torch.zeros(4, 20, dtype=torch.uint8), scales), (torch.zeros(4, 0, dtype=torch.uint8), scales),
+                 (torch.zeros(129, 32, dtype=torch.uint8), scales), (torch.zeros(32, 4, dtype=torch.uint8).t(), scales)):
+        with pytest.raises(ops.KernelError):
+            ops.Mx4Matrix(c, s)
+    m = ops.Mx4Matrix(codes, scales)
+    for call in (lambda: m.dequantize(), lambda: ops.mx4_quantize(torch.zeros(4, 64)),
+                 lambda: ops.linear(torch.zeros(4, 64, dtype=torch.bfloat16), m)):
+        with pytest.raises(ops.KernelError):                             # there is no CPU path
+            call()
+
+
+def test_plain_rounding():
+    """The oracle itself: ties to the even code, at most 6, the scale of a block."""
+    x = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9, -0.25, -0.75, -5.0, 4.0] + [0.0] * 20)
+    _, scales, v = plain.quantize(x[None])
+    assert scales.tolist() == [[127]]
+    assert v[0, :12].tolist() == [0, 1, 1, 2, 2, 4, 4, 6, 0, -1, -4, 4]
+    _, scales, v = plain.quantize((x * 2.0 ** -130)[None])
+    assert scales.tolist() == [[0]] and v[0, 11] == 2.0 ** -128
