@@ -14,8 +14,7 @@
 // The rows of A may be sorted by expert (offsets int32 [E + 1] on the device): expert e's rows form row tiles of their own, counted by
 // every CTA itself, whose scales lie in the same order (rllm_mx4_quantize); its matrix is number e of the stack B.
 // The gated product: B is a stack of gate and up matrices in turn; a tile holds 128 gate rows and the 128 up rows of the same index.
-#include "tcgen05.cuh"
-#include "mx4.cuh"
+#include "mx4_tc.cuh"
 
 #define GM_BM 128
 #define GM_BN 256
@@ -24,40 +23,11 @@
 #define GM_MAX_E 1024
 #define GM_A_BYTES (GM_BM * 128)
 #define GM_B_BYTES (GM_BN * 128)
-#define GM_SF_BYTES (2 * MX4_ATOM)                         // the scales of 128 rows in a stage
-#define GM_STAGE_BYTES (GM_A_BYTES + GM_B_BYTES + 3 * GM_SF_BYTES)
+#define GM_STAGE_BYTES (GM_A_BYTES + GM_B_BYTES + 3 * MX4_SF_BYTES)
 #define GM_SF_COLS 32                                      // tensor-memory columns of a stage's scales: 8 of A, 16 of B
 
 enum { GM_EPI_STORE = 0, GM_EPI_ACCUM = 1, GM_EPI_GATED = 2 };
 enum { GM_ERR_FULL = 31, GM_ERR_EMPTY = 32, GM_ERR_ACC = 33 };
-
-// ---------------------------------------------------------------- the instructions
-// Instruction descriptor of kind mxf4: A and B e2m1 (1), scales ue8m0 (bit 23), both operands K-major, shape M x N x 64; bits 4-5 and
-// 29-30 say which bytes of the scale columns belong to B and A (0 or 2: two scales a row and instruction).
-__host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, int sf_id) {
-    return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | ((uint32_t)sf_id << 4) |
-           ((uint32_t)sf_id << 29);
-}
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                          uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
-// Shared-memory descriptor of one atom of scales: 32 lines of 16 bytes without swizzle, groups of 8 lines 128 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_atom(uint32_t saddr) {
-    return ((uint64_t)((128u >> 4) | (1u << 14)) << 32) | ((saddr & 0x3FFFFu) >> 4);
-}
-// 512 bytes -> four columns, the 32 lines repeated for the four quarters of the lanes
-__device__ __forceinline__ void tmem_cp_atom(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(s_addr(dst)), "l"(src), "r"(bytes), "r"(s_addr(bar)) : "memory");
-}
 
 template <typename TC> __device__ __forceinline__ void gm_store32(TC* dst, const float (&v)[32], int n_valid) {
     if (n_valid >= 32 && ((uintptr_t)dst & 15) == 0) {
@@ -104,7 +74,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkb = (K + MX4_CHUNK - 1) / MX4_CHUNK, n_tiles = (N + BN_OUT - 1) / BN_OUT;
     const int rb_n = (N + 127) >> 7;                 // blocks of 128 scale rows of one matrix of B
-    const size_t rb_bytes = (size_t)nkb * GM_SF_BYTES;
+    const size_t rb_bytes = (size_t)nkb * MX4_SF_BYTES;
     const int rb_most = offsets ? ((rows + GM_BM - 1) / GM_BM + E) : (rows + GM_BM - 1) / GM_BM;
     if (tid == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
@@ -166,21 +136,21 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         bool ok = true;
         auto load_b = [&](int s, int kb, int e, int n0) {
             unsigned char* b_s = smem + (size_t)s * GM_STAGE_BYTES + GM_A_BYTES;
-            unsigned char* f_s = b_s + GM_B_BYTES + GM_SF_BYTES;
+            unsigned char* f_s = b_s + GM_B_BYTES + MX4_SF_BYTES;
             const int rb = n0 >> 7;
             if (GATED) {
                 const long long g = 2ll * e;
                 tma_load_2d(b_s, &tmB, kb * 128, (int)(g * N) + n0, &full_bar[s]);
                 tma_load_2d(b_s + GM_B_BYTES / 2, &tmB, kb * 128, (int)((g + 1) * N) + n0, &full_bar[s]);
-                bulk_load(f_s, sfb + (g * rb_n + rb) * rb_bytes + (size_t)kb * GM_SF_BYTES, GM_SF_BYTES, &full_bar[s]);
-                bulk_load(f_s + GM_SF_BYTES, sfb + ((g + 1) * rb_n + rb) * rb_bytes + (size_t)kb * GM_SF_BYTES, GM_SF_BYTES, &full_bar[s]);
+                bulk_load(f_s, sfb + (g * rb_n + rb) * rb_bytes + (size_t)kb * MX4_SF_BYTES, MX4_SF_BYTES, &full_bar[s]);
+                bulk_load(f_s + MX4_SF_BYTES, sfb + ((g + 1) * rb_n + rb) * rb_bytes + (size_t)kb * MX4_SF_BYTES, MX4_SF_BYTES, &full_bar[s]);
             } else {
                 // (the second 128 rows of a matrix's last tile may not exist: whatever comes in belongs to columns that are dropped)
                 const long long r0 = (long long)e * rb_n;
                 tma_load_2d(b_s, &tmB, kb * 128, e * N + n0, &full_bar[s]);
                 tma_load_2d(b_s + GM_B_BYTES / 2, &tmB, kb * 128, e * N + n0 + 128, &full_bar[s]);
-                bulk_load(f_s, sfb + (r0 + rb) * rb_bytes + (size_t)kb * GM_SF_BYTES, GM_SF_BYTES, &full_bar[s]);
-                bulk_load(f_s + GM_SF_BYTES, sfb + (r0 + min(rb + 1, rb_n - 1)) * rb_bytes + (size_t)kb * GM_SF_BYTES, GM_SF_BYTES,
+                bulk_load(f_s, sfb + (r0 + rb) * rb_bytes + (size_t)kb * MX4_SF_BYTES, MX4_SF_BYTES, &full_bar[s]);
+                bulk_load(f_s + MX4_SF_BYTES, sfb + (r0 + min(rb + 1, rb_n - 1)) * rb_bytes + (size_t)kb * MX4_SF_BYTES, MX4_SF_BYTES,
                           &full_bar[s]);
             }
         };
@@ -210,7 +180,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 unsigned char* a_s = smem + (size_t)s * GM_STAGE_BYTES;
                 if (it >= head) mbar_expect_tx(&full_bar[s], GM_STAGE_BYTES);
                 tma_load_2d(a_s, &tmA, kb * 128, m0, &full_bar[s]);
-                bulk_load(a_s + GM_A_BYTES + GM_B_BYTES, sf_rows + (size_t)kb * GM_SF_BYTES, GM_SF_BYTES, &full_bar[s]);
+                bulk_load(a_s + GM_A_BYTES + GM_B_BYTES, sf_rows + (size_t)kb * MX4_SF_BYTES, MX4_SF_BYTES, &full_bar[s]);
                 if (it >= head) load_b(s, kb, e, n0);
                 issued = it + 1;
             }
@@ -246,8 +216,8 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {                // 128 entries along K each
                     tmem_cp_atom(t_a + 4 * g, smem_desc_atom(f_addr + g * MX4_ATOM));
-                    tmem_cp_atom(t_b + 8 * g, smem_desc_atom(f_addr + GM_SF_BYTES + g * MX4_ATOM));
-                    tmem_cp_atom(t_b + 8 * g + 4, smem_desc_atom(f_addr + 2 * GM_SF_BYTES + g * MX4_ATOM));
+                    tmem_cp_atom(t_b + 8 * g, smem_desc_atom(f_addr + MX4_SF_BYTES + g * MX4_ATOM));
+                    tmem_cp_atom(t_b + 8 * g + 4, smem_desc_atom(f_addr + 2 * MX4_SF_BYTES + g * MX4_ATOM));
                 }
                 const uint64_t a_desc = smem_desc_sw128(a_addr), b_desc = smem_desc_sw128(a_addr + GM_A_BYTES);
 #pragma unroll
@@ -322,19 +292,6 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 }
 
 // ---------------------------------------------------------------- host side
-// Tensor map of codes [rows, k / 2] (contiguous): boxes of box_rows x 128 bytes, 128-byte swizzle, zeros outside.
-static int gm_tmap(CUtensorMap* map, const void* base, long long rows, int k, int box_rows) {
-    TmapEncodeFn enc = tmap_encoder();
-    if (!enc) return 30001;
-    const cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)(k / 2)};
-    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : 30000 + (int)r;
-}
-
 // A: codes [rows, K / 2] and scales; B: codes [matrices * N, K / 2] and the matrices' scales one after another (matrices: E, gated
 // 2 E, gate and up in turn).  K a multiple of 32, all bases 16-byte aligned.  offsets int32 [E + 1] on the device (null: E is 1, all
 // rows are its).  epilogue 0 store, 1 add into a float32 C, 2 gated (GluForm).  ahead: B is settled and may be read before the
@@ -349,9 +306,9 @@ RLLM_API int rllm_gemm_mx4(const void* a_codes, const void* a_scales, const void
         ((uintptr_t)b_scales & 15) || (epilogue == GM_EPI_ACCUM && c_dtype != RLLM_F32))
         return (int)cudaErrorInvalidValue;
     CUtensorMap ta, tb;
-    int st = gm_tmap(&ta, a_codes, rows, K, GM_BM);
+    int st = mx4_tmap(&ta, a_codes, rows, K, GM_BM);
     if (st) return st;
-    st = gm_tmap(&tb, b_codes, matrices * N, K, 128);
+    st = mx4_tmap(&tb, b_codes, matrices * N, K, 128);
     if (st) return st;
     const GluForm glu = GluForm{glu_limit, glu_alpha, glu_shift};
     const int bn_out = epilogue == GM_EPI_GATED ? GM_BN / 2 : GM_BN;

@@ -1473,7 +1473,8 @@ def check_device_errors(device="cuda:0") -> None:
 
 
 _WAIT_LIBRARIES = {"tc": "rllm_tc", "tc2": "rllm_tc2", "stream": "rllm_stream", "attn_tc": "rllm_attn_tc",
-                   "group": "rllm_gemm_group", "mx4_tc": "rllm_gemm_mx4"}
+                   "group": "rllm_gemm_group", "mx4_tc": "rllm_gemm_mx4",
+                   "mx4_rows": "rllm_gemm_mx4_rows"}
 
 
 def set_wait_cycles(cycles: int = 0, libraries=None) -> None:
@@ -2109,6 +2110,37 @@ def _gemm_mx4(codes, scales, w, out, n, epilogue, glu=None, offsets=None, expert
     return out
 
 
+MX4_FEW_ROWS = 64              # up to this many rows a product is one launch that quantises them itself
+
+
+def mx4_row_splits(tiles: int, k: int, n_sm: int = 148) -> int:
+    """CTAs that share the K of a tile of 128 weight rows in the product of few rows."""
+    chunks, s = -(-k // 256), 1
+    while s < 8 and 2 * s <= chunks and tiles * 2 * s <= 2 * n_sm:
+        s *= 2
+    return s
+
+
+def _mx4_few(x) -> bool:
+    return (x.shape[0] <= MX4_FEW_ROWS and x.data_ptr() % 16 == 0
+            and (x.shape[0] == 1 or x.stride(0) * x.element_size() % 16 == 0))
+
+
+def _gemm_mx4_rows(x, w, out, n, epilogue, glu=None, splits=None):
+    limit, alpha, shift = glu or (0.0, 1.0, 0.0)
+    m, k = x.shape
+    if splits is None:
+        splits = mx4_row_splits(-(-n // 128), k, sm_count(x.device))
+    st = _lib("mx4_rows").rllm_gemm_mx4_rows(
+        _ptr(x), c_int(_code(x)), c_longlong(x.stride(0) if m > 1 else 0), _ptr(w.codes), _ptr(w.scales), _ptr(out), c_int(_code(out)),
+        c_longlong(out.stride(0) if m > 1 else n), c_int(m), c_int(n), c_int(k), c_int(epilogue), c_int(splits), c_int(1 if w.settled else 0), c_float(limit),
+        c_float(alpha), c_float(shift), _ptr(error_word(x.device)), _stream())
+    if st >= 30000:
+        raise KernelError(f"gemm_mx4_rows: tensor map encoding failed (CUresult {st - 30000})")
+    _check(st, "gemm_mx4_rows")
+    return out
+
+
 def _mx4_product(x, w, out, n, lead, who):
     """Checks that the products have in common: x [m, k], w a stack `lead` of [n, k], out [m, n]."""
     _need_cuda(x, w, out)
@@ -2134,7 +2166,10 @@ def mx4_linear(x, w, out=None, out_dtype=None, accumulate=False):
     if accumulate and out.dtype != torch.float32:
         raise KernelError("accumulating product needs a float32 output")
     if m and n:
-        _gemm_mx4(*_mx4_operand(x, "mx4_linear"), w, out, n, EPI_ACCUM if accumulate else EPI_STORE)
+        epilogue = EPI_ACCUM if accumulate else EPI_STORE
+        if _mx4_few(x):
+            return _gemm_mx4_rows(x, w, out, n, epilogue)
+        _gemm_mx4(*_mx4_operand(x, "mx4_linear"), w, out, n, epilogue)
     return out
 
 
@@ -2146,6 +2181,8 @@ def mx4_gated(h, w, out, glu=None):
     if h.shape[0] != m:
         raise KernelError(f"mx4_gated: an output of {m} rows for {h.shape[0]}")
     if m and F:
+        if _mx4_few(h):
+            return _gemm_mx4_rows(h, w, out, F, EPI_SWIGLU, glu)
         _gemm_mx4(*_mx4_operand(h, "mx4_gated"), w, out, F, EPI_SWIGLU, glu)
     return out
 

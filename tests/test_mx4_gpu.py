@@ -374,3 +374,31 @@ def test_offsets_that_do_not_rise():
     torch.cuda.synchronize()
     assert bool((act[300:] == 5.0).all())
     o.check_device_errors()
+
+
+@pytest.mark.parametrize("splits", [1, 2, 4, 8])
+@pytest.mark.parametrize("m", [1, 2, 7, 16, 17, 40, 64])
+@pytest.mark.parametrize("n,k", [(200, 2080), (128, 256), (1000, 8192)])
+def test_few_rows_shared_k(m, n, k, splits):
+    """Every way to share K, also between more CTAs than there are chunks of K; float32 rows; a ring that wraps."""
+    o = ops()
+    w, values = weight(n, k, seed=1)
+    g, gv = weight(2, n, k, seed=2)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = rnd(m, k, seed=3, dtype=dtype)
+        xq = plain.quantize(x)[2]
+        want, size = plain.product(xq, values)
+        slack = plain.product_slack(size, k)
+        out = torch.full((m + 1, n + 2), 5.0, device=DEV)
+        o._gemm_mx4_rows(x, w, out[:m, :n], n, o.EPI_STORE, splits=splits)
+        plain.near(out[:m, :n], want, slack)
+        c = rnd(m, n, seed=4)
+        out[:m, :n] = c
+        o._gemm_mx4_rows(x, w, out[:m, :n], n, o.EPI_ACCUM, splits=splits)
+        plain.near(out[:m, :n], want + c.double(), slack + 2.0 ** -24 * (want.abs() + c.double().abs()))
+        out[:m, :n] = 5.0
+        assert bool((out == 5.0).all())
+        act = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+        o._gemm_mx4_rows(x, g, act, n, o.EPI_SWIGLU, glu=CLAMPED, splits=splits)
+        plain.near(act, *plain.gated(xq, gv[0], gv[1], CLAMPED))
+    o.check_device_errors()
