@@ -44,8 +44,7 @@ LIBRARIES = {
     "tc2": (["gemm_tc2.cu"], []),
     "group": (["gemm_group.cu"], []),
     "stream": (["gemv_stream.cu"], []),
-    "mx4": (["mx4.cu"], []),
-    "mx4_tc": (["gemm_mx4.cu"], []),
+    "mx4": (["mx4.cu", "gemm_mx4.cu"], []),
     "mx4_rows": (["gemm_mx4_rows.cu"], []),
     "attn_tc": (["attention_tc.cu"], []),
     "host": (["host_runtime.cpp"], []),

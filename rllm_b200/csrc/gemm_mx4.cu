@@ -16,6 +16,10 @@
 // The gated product: B is a stack of gate and up matrices in turn; a tile holds 128 gate rows and the 128 up rows of the same index.
 #include "mx4_tc.cuh"
 
+// mx4.cu
+RLLM_API int rllm_mx4_quantize(const void* x, void* codes, void* scales, const int* offsets, const int* place, long long ld, int dt,
+                               int rows, int k, int pad, int E, int top_k, cudaStream_t stream);
+
 #define GM_BM 128
 #define GM_BN 256
 #define GM_STAGES 4
@@ -296,7 +300,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 // 2 E, gate and up in turn).  K a multiple of 32, all bases 16-byte aligned.  offsets int32 [E + 1] on the device (null: E is 1, all
 // rows are its).  epilogue 0 store, 1 add into a float32 C, 2 gated (GluForm).  ahead: B is settled and may be read before the
 // kernels before have ended.  Returns 0, a cudaError_t or 30000 + CUresult of the tensor-map encoder.
-RLLM_API int rllm_gemm_mx4(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales, void* C, int c_dtype,
+static int rllm_gemm_mx4(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales, void* C, int c_dtype,
                            long long ldc, const int* offsets, int E, int rows, int N, int K, int epilogue, int ahead, float glu_limit,
                            float glu_alpha, float glu_shift, int* err, cudaStream_t stream) {
     if (rows <= 0 || N <= 0) return 0;
@@ -332,4 +336,17 @@ RLLM_API int rllm_gemm_mx4(const void* a_codes, const void* a_scales, const void
 
 TC_DEFINE_WAIT_CONTROLS(rllm_gemm_mx4)
 
-RLLM_PACKED(rllm_gemm_mx4)
+// The whole product from rows x [rows of x, K] (float32 or bfloat16, ldx apart): they are quantised into `work` (codes, and from the next multiple
+// of 1,024 bytes the scales), which rllm_gemm_mx4 then reads.  offsets, place, E, top_k as for rllm_mx4_quantize; `rows` sorted rows.
+RLLM_API int rllm_mx4_product(const void* x, const int* offsets, const int* place, const void* w_codes, const void* w_scales, void* C,
+                              void* work, int* err, long long ldx, long long ldc, int x_dtype, int c_dtype, int rows, int N, int K, int E,
+                              int top_k, int epilogue, int ahead, float glu_limit, float glu_alpha, float glu_shift, cudaStream_t stream) {
+    if (rows <= 0 || N <= 0) return 0;
+    unsigned char* scales = (unsigned char*)work + (((size_t)rows * (size_t)(K / 2) + 1023) & ~(size_t)1023);
+    const int st = rllm_mx4_quantize(x, work, scales, offsets, place, ldx, x_dtype, rows, K, 0, E, top_k, stream);
+    if (st) return st;
+    return rllm_gemm_mx4(work, scales, w_codes, w_scales, C, c_dtype, ldc, offsets, E, rows, N, K, epilogue, ahead, glu_limit, glu_alpha,
+                         glu_shift, err, stream);
+}
+
+RLLM_PACKED(rllm_mx4_product)

@@ -22,14 +22,7 @@ template <> struct RowPart<bf16> {
     uint4 u;
     __device__ __forceinline__ void load(const bf16* p) { u = *reinterpret_cast<const uint4*>(p); }
     __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
+    __device__ __forceinline__ void get(float (&v)[8]) const { mx4_unpack(u, v); }
 };
 template <> struct RowPart<float> {
     float4 a, b;
@@ -179,18 +172,10 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const uint8_t* sfw
                         if (ok) {
                             float f[8];
                             part[u].get(f);
-                            uint32_t top = mx4_top8(f);
-                            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                            const uint32_t sc = mx4_scale_of(top);
-                            const float inv = mx4_inverse(sc);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) f[j] = sc == 255u ? 0.f : f[j] * inv;
-                            uint32_t word = sc << (8 * ((lane >> 2) & 3));
-                            word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                            word |= __shfl_xor_sync(0xffffffffu, word, 8);
+                            uint32_t word;
+                            const uint32_t code = mx4_quantize8(f, lane, word);
                             unsigned char* x_s = smem + (size_t)s * STAGE_BYTES + WT * W_BYTES;
-                            *reinterpret_cast<uint32_t*>(x_s + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) = mx4_encode8(f);
+                            *reinterpret_cast<uint32_t*>(x_s + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) = code;
                             if ((lane & 15) == 0)
                                 *reinterpret_cast<uint32_t*>(x_s + X_BYTES + WT * MX4_SF_BYTES + (lane >> 4) * MX4_ATOM + (r & 31) * 16 +
                                                              (r >> 5) * 4) = word;
@@ -322,9 +307,9 @@ static int gr_launch(const CUtensorMap& tw, const void* sfw, const void* X, long
 
 // X [m, K] (m <= 64, rows ldx apart, 16-byte aligned rows) in float32 or bfloat16; W: codes [n, K / 2] and scales, gated: gate and up
 // matrix of n rows each.  splits: 1, 2, 4 or 8 CTAs share a tile's K.  The rest as rllm_gemm_mx4.
-RLLM_API int rllm_gemm_mx4_rows(const void* X, int x_dtype, long long ldx, const void* w_codes, const void* w_scales, void* C, int c_dtype,
-                                long long ldc, int m, int n, int K, int epilogue, int splits, int ahead, float glu_limit, float glu_alpha,
-                                float glu_shift, int* err, cudaStream_t stream) {
+RLLM_API int rllm_gemm_mx4_rows(const void* X, const void* w_codes, const void* w_scales, void* C, int* err, long long ldx, long long ldc,
+                                int x_dtype, int c_dtype, int m, int n, int K, int epilogue, int splits, int ahead, float glu_limit,
+                                float glu_alpha, float glu_shift, cudaStream_t stream) {
     if (m <= 0 || n <= 0) return 0;
     const bool gated = epilogue == GR_EPI_GATED;
     if (m > 64 || K <= 0 || (K % MX4_BLOCK) || !err || ldc < n || (long long)n > 0x3fffff00LL || ((uintptr_t)w_codes & 15) ||

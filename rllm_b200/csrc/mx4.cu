@@ -6,94 +6,136 @@
 //                   row tiles: expert e's rows begin a new block of 128 scale rows, the one behind the blocks of the experts before it.
 //   mx4_dequantize  the values that codes and scales stand for, exact in float32 and in bfloat16.
 //
-// Both read and write every byte once; a warp takes 256 neighbouring entries of a row, a lane eight of them, so that loads are
-// 512 or 1,024 and code stores 128 contiguous bytes; the four lanes of a block find its largest magnitude with two shuffles.
+// Both read and write every byte once; a warp takes up to four runs of 256 neighbouring entries of a row (all their loads in flight at
+// once), a lane eight entries of each, so that loads are 512 or 1,024 and code stores 128 contiguous bytes; the four lanes of a block
+// find its largest magnitude with two shuffles.
 #include "mx4.cuh"
+
+#define MQ_RUNS 4                            // runs of 256 entries of a warp
+
+template <typename T> struct MqPart;
+template <> struct MqPart<bf16> {
+    uint4 u;
+    template <bool VEC> __device__ __forceinline__ void load(const bf16* p) {
+        if (VEC) { u = *reinterpret_cast<const uint4*>(p); return; }
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+        u = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+    }
+    __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void get(float (&v)[8]) const { mx4_unpack(u, v); }
+};
+template <> struct MqPart<float> {
+    float v8[8];
+    template <bool VEC> __device__ __forceinline__ void load(const float* p) { mx4_load8<VEC>(p, v8); }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v8[i] = 0.f;
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v8[i];
+    }
+};
 
 template <typename T, bool VEC, bool SORTED>
 __global__ void __launch_bounds__(128)
-mx4_quantize_kernel(const T* x, long long ld, int rows, int k, uint8_t* codes, uint8_t* scales, int pad_rows,
+mx4_quantize_kernel(const T* x, long long ld, int rows, int k, uint8_t* codes, uint8_t* scales, unsigned n_warps, unsigned per_row,
                     const int* offsets, const int* place, int E, int top_k) {
     // the kernels behind may start once the ones before are complete: a product reads its weights ahead of its own wait, and
     // those may be what the kernel before this one wrote
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int chunks = (k + MX4_CHUNK - 1) / MX4_CHUNK;
-    const long long kg = 2 * (long long)chunks;
-    const long long n_warps = (long long)gridDim.x * (blockDim.x >> 5);
-    for (long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < (long long)pad_rows * chunks; w += n_warps) {
-        const long long item = w / chunks;
-        const int c = (int)(w - item * chunks), col = c * MX4_CHUNK + lane * 8;
-        long long src = item, row = item, scale_row = item;
-        if (SORTED) {
-            if (place) {
-                row = place[item];
-                src = item / top_k;
-                if (row < 0 || row >= rows) continue;
-            }
-            // the row's expert: the last one that begins at or before it; and the row tiles of the experts before that one
-            int lo = 0, hi = E;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (offsets[mid] <= row) lo = mid; else hi = mid;
-            }
-            int tiles = 0;
-            for (int e = lane; e < lo; e += 32) tiles += (offsets[e + 1] - offsets[e] + 127) >> 7;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-            scale_row = (long long)tiles * 128 + (row - offsets[lo]);
-            // (offsets that do not rise from 0 to the number of rows: nothing outside the scales is written)
-            if (scale_row < 0 || scale_row >= ((long long)((rows + 127) >> 7) + E) * 128) continue;
+    const unsigned w = blockIdx.x * 4u + (threadIdx.x >> 5);
+    if (w >= n_warps) return;
+    const unsigned item = w / per_row;
+    const int chunks = (k + MX4_CHUNK - 1) / MX4_CHUNK, c0 = (int)(w - item * per_row) * MQ_RUNS;
+    long long src = item, row = item, scale_row = item;
+    if (SORTED) {
+        if (place) {
+            row = place[item];
+            src = item / (unsigned)top_k;
+            if (row < 0 || row >= rows) return;
         }
+    }
+    MqPart<T> part[MQ_RUNS];
+    const bool here = item < (unsigned)rows;                     // (rows behind the last one get scales of zero)
+#pragma unroll
+    for (int i = 0; i < MQ_RUNS; ++i) {
+        const int col = (c0 + i) * MX4_CHUNK + lane * 8;         // (k is a multiple of 32: a lane's eight are all in or all out)
+        if (here && col < k) part[i].template load<VEC>(x + src * ld + col);
+        else part[i].zero();
+    }
+    if (SORTED) {
+        // the row's expert is the first that ends behind it; its rows begin behind the row tiles of the experts before
+        int before = 0, tiles = 0;
+        for (int e = lane; e < E; e += 32) {
+            const int end = offsets[e + 1];
+            if (end <= row) {
+                ++before;
+                tiles += (end - offsets[e] + 127) >> 7;
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+            tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        }
+        if (before >= E) return;
+        scale_row = (long long)tiles * 128 + (row - offsets[before]);
+        // (offsets that do not rise from 0 to the number of rows: nothing outside the scales is written)
+        if (scale_row < 0 || scale_row >= ((long long)((rows + 127) >> 7) + E) * 128) return;
+    }
+#pragma unroll
+    for (int i = 0; i < MQ_RUNS; ++i) {
+        const int c = c0 + i, col = c * MX4_CHUNK + lane * 8;
+        if (c >= chunks) break;
         float v[8];
-        const bool in = item < rows && col < k;                  // (k is a multiple of 32: a lane's eight are all in or all out)
-        if (in) mx4_load8<VEC>(x + src * ld + col, v);
-        else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        }
-        uint32_t top = mx4_top8(v);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t s = mx4_scale_of(top);
-        const float inv = mx4_inverse(s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = s == 255u ? 0.f : v[i] * inv;
-        if (in) *reinterpret_cast<uint32_t*>(codes + row * (long long)(k >> 1) + (col >> 1)) = mx4_encode8(v);
-        // the four scales of 128 entries as one word
-        uint32_t word = s << (8 * ((lane >> 2) & 3));
-        word |= __shfl_xor_sync(0xffffffffu, word, 4);
-        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+        part[i].get(v);
+        uint32_t word;
+        const uint32_t code = mx4_quantize8(v, lane, word);
+        if (here && col < k) *reinterpret_cast<uint32_t*>(codes + row * (long long)(k >> 1) + (col >> 1)) = code;
         if ((lane & 15) == 0)
-            *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(scale_row, (long long)c * 8 + (lane >> 4) * 4, kg)) = word;
+            *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(scale_row, (long long)c * 8 + (lane >> 4) * 4, 2ll * chunks)) = word;
     }
 }
 
 // A stack of matrices: `rows` rows each, whose scales take rb * 128 scale rows.
 template <typename T>
 __global__ void __launch_bounds__(128)
-mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, long long all_rows, int rows, int k, T* out) {
+mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, unsigned rows, int k, T* out, unsigned n_warps, unsigned per_row) {
     pdl_wait();
     pdl_launch_dependents();
-    const long long kg = mx4_atoms_k(k), rb = (rows + 127) / 128, per = k >> 3, n = all_rows * per;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const long long row = i / per, g = row / rows, r = row - g * rows;
-        const int col = (int)(i - row * per) * 8;
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + i * 4);
-        const uint32_t s = scales[(size_t)g * rb * kg * MX4_ATOM + mx4_scale_at(r, col >> 5, kg)];
-        const float f = s == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(s ? s << 23 : 0x00400000u);
+    const int lane = threadIdx.x & 31;
+    const unsigned w = blockIdx.x * 4u + (threadIdx.x >> 5);
+    if (w >= n_warps) return;
+    const unsigned row = w / per_row, g = row / rows, r = row - g * rows;
+    const int c0 = (int)(w - row * per_row) * MQ_RUNS;
+    const long long kg = mx4_atoms_k(k), base = (long long)row * k;
+    const uint8_t* sc = scales + (size_t)g * ((rows + 127) >> 7) * kg * MX4_ATOM;
+    uint32_t word[MQ_RUNS], s[MQ_RUNS];
+#pragma unroll
+    for (int i = 0; i < MQ_RUNS; ++i) {
+        const int col = (c0 + i) * MX4_CHUNK + lane * 8;
+        word[i] = col < k ? *reinterpret_cast<const uint32_t*>(codes + ((base + col) >> 1)) : 0u;
+        s[i] = col < k ? sc[mx4_scale_at(r, col >> 5, kg)] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < MQ_RUNS; ++i) {
+        const int col = (c0 + i) * MX4_CHUNK + lane * 8;
+        if (col >= k) break;
+        const float f = s[i] == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(s[i] ? s[i] << 23 : 0x00400000u);
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t c = (word >> (4 * j)) & 15u, e = (c >> 1) & 3u, m = c & 1u;
-            // e2m1 as float32: 0.5 m for exponent 0, else 2^(e - 1) (1 + m / 2)
-            const uint32_t bits = e ? ((e + 126u) << 23) | (m << 22) : (m ? 0x3f000000u : 0u);
-            v[j] = __uint_as_float(bits | ((c & 8u) << 28)) * f;
+            // the three bits of the magnitude as a float32's lowest exponent bits and highest mantissa bit: the number times 2^-126
+            const uint32_t mag = (j <= 5 ? word[i] << (22 - 4 * j) : word[i] >> (4 * j - 22)) & 0x01c00000u;
+            v[j] = __uint_as_float(mag | ((word[i] << (28 - 4 * j)) & 0x80000000u)) * 8.507059173023462e37f * f;
         }
+        T* o = out + base + col;
         if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4*>(out + i * 8)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(out + i * 8)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
         } else {
             uint32_t u[4];
 #pragma unroll
@@ -101,29 +143,37 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, long long all
                 const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
                 u[j] = *reinterpret_cast<const uint32_t*>(&b);
             }
-            *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[2], u[3]);
         }
     }
+}
+
+// Warps for `rows` rows of k entries: how many a row takes, and all of them (0: more than one launch can have).
+static unsigned mq_warps(long long rows, int k, unsigned& per_row) {
+    per_row = (unsigned)((k + MX4_CHUNK * MQ_RUNS - 1) / (MX4_CHUNK * MQ_RUNS));
+    const long long n = rows * per_row;
+    return n < 0xfffffff0ll ? (unsigned)n : 0u;
 }
 
 template <typename T, bool VEC>
 static int mx4_launch(const T* x, long long ld, int rows, int k, uint8_t* codes, uint8_t* scales, int pad_rows, const int* offsets,
                       const int* place, int E, int top_k, cudaStream_t stream) {
-    const long long warps = (long long)pad_rows * ((k + MX4_CHUNK - 1) / MX4_CHUNK), blocks = (warps + 3) / 4;
-    const long long most = 16ll * rllm_sm_count();
-    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    unsigned per_row;
+    const unsigned n = mq_warps(pad_rows, k, per_row);
+    if (!n) return (int)cudaErrorInvalidValue;
+    const dim3 grid(n / 4 + (n % 4 != 0));
     if (offsets)
-        return rllm_launch(mx4_quantize_kernel<T, VEC, true>, grid, dim3(128), 0, stream, x, ld, rows, k, codes, scales, pad_rows,
+        return rllm_launch(mx4_quantize_kernel<T, VEC, true>, grid, dim3(128), 0, stream, x, ld, rows, k, codes, scales, n, per_row,
                            offsets, place, E, top_k);
-    return rllm_launch(mx4_quantize_kernel<T, VEC, false>, grid, dim3(128), 0, stream, x, ld, rows, k, codes, scales, pad_rows,
+    return rllm_launch(mx4_quantize_kernel<T, VEC, false>, grid, dim3(128), 0, stream, x, ld, rows, k, codes, scales, n, per_row,
                        offsets, place, E, top_k);
 }
 
 // x [rows, k] with rows ld apart -> codes [rows, k / 2] (16-byte aligned), scales.  k a multiple of 32.  pad != 0: the scales of
 // the rows behind the last one, up to a multiple of 128, are written too (zeros).  offsets int32 [E + 1] (sorted rows, see
 // above): then `rows` is the number of sorted rows and `place`, if given, int32 [rows].
-RLLM_API int rllm_mx4_quantize(const void* x, int dt, long long ld, int rows, int k, void* codes, void* scales, int pad,
-                               const int* offsets, const int* place, int E, int top_k, cudaStream_t stream) {
+RLLM_API int rllm_mx4_quantize(const void* x, void* codes, void* scales, const int* offsets, const int* place, long long ld, int dt,
+                               int rows, int k, int pad, int E, int top_k, cudaStream_t stream) {
     if (rows <= 0 || k <= 0) return 0;
     if ((k % MX4_BLOCK) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15) || (offsets && (E <= 0 || pad)) || (place && top_k <= 0) ||
         (place && !offsets) || rows > 0x7fffff00)
@@ -140,17 +190,18 @@ RLLM_API int rllm_mx4_quantize(const void* x, int dt, long long ld, int rows, in
 }
 
 // out [matrices * rows, k] contiguous, float32 or bfloat16, 16-byte aligned
-RLLM_API int rllm_mx4_dequantize(const void* codes, const void* scales, long long matrices, int rows, int k, void* out, int dt,
+RLLM_API int rllm_mx4_dequantize(const void* codes, const void* scales, void* out, long long matrices, int rows, int k, int dt,
                                  cudaStream_t stream) {
     if (matrices <= 0 || rows <= 0 || k <= 0) return 0;
-    if ((k % MX4_BLOCK) || ((uintptr_t)codes & 3) || ((uintptr_t)out & 15)) return (int)cudaErrorInvalidValue;
-    const long long blocks = (matrices * rows * (k / 8) + 127) / 128, most = 16ll * rllm_sm_count();
-    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    unsigned per_row;
+    const unsigned n = mq_warps(matrices * rows, k, per_row);
+    if ((k % MX4_BLOCK) || ((uintptr_t)codes & 3) || ((uintptr_t)out & 15) || !n) return (int)cudaErrorInvalidValue;
+    const dim3 grid(n / 4 + (n % 4 != 0));
     if (dt == RLLM_F32)
         return rllm_launch(mx4_dequantize_kernel<float>, grid, dim3(128), 0, stream, (const uint8_t*)codes, (const uint8_t*)scales,
-                           matrices * rows, rows, k, (float*)out);
+                           (unsigned)rows, k, (float*)out, n, per_row);
     return rllm_launch(mx4_dequantize_kernel<bf16>, grid, dim3(128), 0, stream, (const uint8_t*)codes, (const uint8_t*)scales,
-                       matrices * rows, rows, k, (bf16*)out);
+                       (unsigned)rows, k, (bf16*)out, n, per_row);
 }
 
 RLLM_PACKED(rllm_mx4_quantize)

@@ -52,21 +52,32 @@ __device__ __forceinline__ uint32_t mx4_top8(const float (&v)[8]) {
     return t;
 }
 
-// Eight neighbouring entries of a row as float32 (p + 7 inside the row; 16-byte aligned for VEC).
-template <bool VEC> __device__ __forceinline__ void mx4_load8(const bf16* p, float (&v)[8]) {
-    if (VEC) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight neighbouring entries of one lane, the four lanes of a block side by side: their codes, and in `word` the four scale bytes of
+// the 128 entries of the lane's sixteen neighbours.  `v` is used up.
+__device__ __forceinline__ uint32_t mx4_quantize8(float (&v)[8], int lane, uint32_t& word) {
+    uint32_t top = mx4_top8(v);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t s = mx4_scale_of(top);
+    const float inv = mx4_inverse(s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    } else {
+    for (int i = 0; i < 8; ++i) v[i] = s == 255u ? 0.f : v[i] * inv;
+    word = s << (8 * ((lane >> 2) & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    return mx4_encode8(v);
+}
+
+// Eight bfloat16 as float32.
+__device__ __forceinline__ void mx4_unpack(const uint4 u, float (&v)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f<bf16>(p[i]);
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
+// Eight neighbouring float32 (p 16-byte aligned for VEC).
 template <bool VEC> __device__ __forceinline__ void mx4_load8(const float* p, float (&v)[8]) {
     if (VEC) {
         const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];

@@ -243,6 +243,29 @@ def core():
     return _lib("core")
 
 
+class _Packed:
+    """A launcher called through its packed form (common.cuh): its arguments as 64-bit words in one buffer, which costs the host a
+    third of a conversion per argument (19 arguments: 2 us against 6).  The launcher takes its pointers first, then integers, then
+    floats, the stream last.  While launches are recorded or timed it is called as the others are."""
+
+    def __init__(self, library, name, pointers, integers, floats=0):
+        self.library, self.name = library, name
+        self._pack = struct.Struct("<" + "Q" * pointers + "q" * integers + "f4x" * floats + "Q").pack
+        self._integers, self._fn = integers, None
+
+    def __call__(self, tensors, integers, floats=()):
+        if _trace is None and self._fn is not None:
+            return self._fn(self._pack(*[0 if t is None else t.data_ptr() for t in tensors], *integers, *floats,
+                                       _raw_stream(_current_device())))
+        lib = _lib(self.library)
+        if _trace is None and not profiler.enabled():
+            self._fn = getattr(lib, self.name + "_packed")
+            self._fn.argtypes = [ctypes.c_char_p]
+            return self(tensors, integers, floats)
+        return getattr(lib, self.name)(*[_ptr(t) for t in tensors], *[c_longlong(i) for i in integers], *[c_float(f) for f in floats],
+                                       _stream())
+
+
 # ------------------------------------------------------------------ elementwise
 
 def embed(table, tokens, out, err=None, scale=1.0):
@@ -1473,7 +1496,7 @@ def check_device_errors(device="cuda:0") -> None:
 
 
 _WAIT_LIBRARIES = {"tc": "rllm_tc", "tc2": "rllm_tc2", "stream": "rllm_stream", "attn_tc": "rllm_attn_tc",
-                   "group": "rllm_gemm_group", "mx4_tc": "rllm_gemm_mx4",
+                   "group": "rllm_gemm_group", "mx4": "rllm_gemm_mx4",
                    "mx4_rows": "rllm_gemm_mx4_rows"}
 
 
@@ -1966,19 +1989,22 @@ class Mx4Matrix:
 
     `linear` and `gate_up_swiglu` take one in place of a weight.  settled: the caller knows that no kernel that writes codes or scales is still
     in flight (the weights of a loaded model); products may then read them before the kernels launched before have ended."""
-    __slots__ = ("codes", "scales", "settled")
+    __slots__ = ("codes", "scales", "settled", "shape", "device", "is_cuda")
+    dtype = torch.uint8
 
     def __init__(self, codes, scales, settled=False):
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 2 or scales.dim() != codes.dim() + 3:
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.dim() < 2 or scales.dim() != codes.dim() + 3:
             raise KernelError("Mx4Matrix: codes are uint8 [..., n, k / 2], scales uint8 [..., n / 128, k / 128, 32, 4, 4]")
-        n, k = codes.shape[-2], 2 * codes.shape[-1]
+        *lead, n, half = codes.shape
+        k = 2 * half
         if k % MX4_BLOCK or k == 0:
             raise KernelError(f"Mx4Matrix: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
-        if scales.shape != codes.shape[:-2] + mx4_scale_shape(n, k) or scales.device != codes.device:
+        if tuple(scales.shape) != (*lead, -(-n // 128), 2 * -(-k // 256), 32, 4, 4) or scales.device != codes.device:
             raise KernelError(f"Mx4Matrix: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)}")
         if not codes.is_contiguous() or not scales.is_contiguous() or (codes.data_ptr() | scales.data_ptr()) % 16:
             raise KernelError("Mx4Matrix: codes and scales must be contiguous and begin at a multiple of 16 bytes")
         self.codes, self.scales, self.settled = codes, scales, settled
+        self.shape, self.device, self.is_cuda = (*lead, n, k), codes.device, codes.is_cuda
 
     @classmethod
     def from_blocks(cls, codes, scales, settled=False):
@@ -2001,40 +2027,16 @@ class Mx4Matrix:
 
     def dequantize(self, dtype=torch.float32):
         """The values [..., n, k] (exact in float32 and in bfloat16)."""
-        _need_cuda(self.codes, self.scales)
+        _need_cuda(self)
+        _mx4_current(self)
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        n, k = self.shape[-2:]
-        if out.numel():
-            _mx4_current(self)
-            _check(_lib("mx4").rllm_mx4_dequantize(_ptr(self.codes), _ptr(self.scales), c_longlong(self.matrices), c_int(n), c_int(k),
-                                                   _ptr(out), c_int(_code(out)), _stream()), "mx4_dequantize")
-        return out
-
-    @property
-    def shape(self):
-        return self.codes.shape[:-1] + (2 * self.codes.shape[-1],)
-
-    @property
-    def matrices(self):
+        code = _code(out)
+        *lead, n, k = self.shape
         m = 1
-        for s in self.codes.shape[:-2]:
+        for s in lead:
             m *= s
-        return m
-
-    @property
-    def dtype(self):
-        return self.codes.dtype
-
-    @property
-    def device(self):
-        return self.codes.device
-
-    @property
-    def is_cuda(self):
-        return self.codes.is_cuda
-
-    def tensors(self):
-        return self.codes, self.scales
+        _check(_mx4_dequantize((self.codes, self.scales, out), (m, n, k, code)), "mx4_dequantize")
+        return out
 
 
 def mx4_scale_shape(n: int, k: int) -> tuple:
@@ -2042,26 +2044,28 @@ def mx4_scale_shape(n: int, k: int) -> tuple:
     return (-(-n // 128), 2 * -(-k // 256), 32, 4, 4)
 
 
+_mx4_quantize = _Packed("mx4", "rllm_mx4_quantize", 5, 7)
+_mx4_dequantize = _Packed("mx4", "rllm_mx4_dequantize", 3, 4)
+_mx4_many = _Packed("mx4", "rllm_mx4_product", 8, 11, 3)
+_mx4_few = _Packed("mx4_rows", "rllm_gemm_mx4_rows", 5, 10, 3)
+
+
 def _mx4_current(*ts):
     """The launchers take the current device's stream: every operand has to be there."""
+    here = _current_device()
     for t in ts:
-        if t is not None and t.device.index not in (None, _current_device()):
-            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{_current_device()}")
+        if t is not None and t.device.index != here:
+            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{here}")
 
 
 def _mx4_rows(x, who):
-    if x.dim() != 2 or x.stride(1) != 1:
+    """(rows, entries, stride of the rows) of x [m, k]."""
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise KernelError(f"{who}: rows [m, k] with neighbouring entries side by side, got {tuple(x.shape)} with strides {x.stride()}")
-    if x.shape[1] % MX4_BLOCK or x.shape[1] == 0:
-        raise KernelError(f"{who}: rows of {x.shape[1]} entries are not whole blocks of {MX4_BLOCK}")
-    return x
-
-
-def _mx4_quantize(x, codes, scales, pad, offsets=None, place=None, experts=0, top_k=0):
-    rows = codes.shape[0]
-    _check(_lib("mx4").rllm_mx4_quantize(_ptr(x), c_int(_code(x)), c_longlong(x.stride(0)), c_int(rows), c_int(x.shape[1]), _ptr(codes),
-                                         _ptr(scales), c_int(pad), _ptr(offsets), _ptr(place), c_int(experts), c_int(top_k), _stream()),
-           "mx4_quantize")
+    m, k = x.shape
+    if k % MX4_BLOCK or k == 0:
+        raise KernelError(f"{who}: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
+    return m, k, x.stride(0)
 
 
 def mx4_quantize(x):
@@ -2070,44 +2074,22 @@ def mx4_quantize(x):
     with an infinity or a NaN becomes NaN.  See mx4.cuh."""
     _need_cuda(x)
     _mx4_current(x)
+    code = _code(x)
     if x.dim() > 2:
         _need_contig(x=x)
-    _mx4_rows(x if x.dim() <= 2 else x.view(-1, x.shape[-1]), "mx4_quantize")
-    *lead, n, k = x.shape
+    m, k, ld = _mx4_rows(x if x.dim() <= 2 else x.view(-1, x.shape[-1]), "mx4_quantize")
+    *lead, n, _ = x.shape
     codes = torch.empty((*lead, n, k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(tuple(lead) + mx4_scale_shape(n, k), dtype=torch.uint8, device=x.device)
-    if x.numel():
-        if x.dim() == 2:
-            _mx4_quantize(x, codes, scales, 1)
-        elif n % 128 == 0:                             # the stack is one matrix as far as rows and scale rows go
-            _mx4_quantize(x.view(-1, k), codes.view(-1, k // 2), scales, 1)
-        else:                                          # every matrix has scale rows of its own
-            c, s = codes.view(-1, n, k // 2), scales.view(-1, *scales.shape[-5:])
-            for i, m in enumerate(x.view(-1, n, k)):
-                _mx4_quantize(m, c[i], s[i], 1)
+    scales = torch.empty((*lead, *mx4_scale_shape(n, k)), dtype=torch.uint8, device=x.device)
+    if m == 0:
+        pass
+    elif not lead or n % 128 == 0:                     # a stack of whole scale blocks is one matrix as far as the kernel goes
+        _check(_mx4_quantize((x, codes, scales, None, None), (ld, code, m, k, 1, 0, 0)), "mx4_quantize")
+    else:
+        parts = codes.view(-1, n, k // 2), scales.view(-1, *scales.shape[-5:])
+        for rows, c, s in zip(x.view(-1, n, k), *parts):
+            _check(_mx4_quantize((rows, c, s, None, None), (k, code, n, k, 1, 0, 0)), "mx4_quantize")
     return Mx4Matrix(codes, scales)
-
-
-def _mx4_operand(x, who):
-    """Rows as a product's first operand: (codes, scales); nothing behind the last row is written."""
-    _mx4_rows(x, who)
-    m, k = x.shape
-    codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(mx4_scale_shape(m, k), dtype=torch.uint8, device=x.device)
-    _mx4_quantize(x, codes, scales, 0)
-    return codes, scales
-
-
-def _gemm_mx4(codes, scales, w, out, n, epilogue, glu=None, offsets=None, experts=1):
-    limit, alpha, shift = glu or (0.0, 1.0, 0.0)
-    st = _lib("mx4_tc").rllm_gemm_mx4(
-        _ptr(codes), _ptr(scales), _ptr(w.codes), _ptr(w.scales), _ptr(out), c_int(_code(out)), c_longlong(out.stride(0)), _ptr(offsets),
-        c_int(experts), c_int(codes.shape[0]), c_int(n), c_int(2 * codes.shape[1]), c_int(epilogue), c_int(1 if w.settled else 0),
-        c_float(limit), c_float(alpha), c_float(shift), _ptr(error_word(codes.device)), _stream())
-    if st >= 30000:
-        raise KernelError(f"gemm_mx4: tensor map encoding failed (CUresult {st - 30000})")
-    _check(st, "gemm_mx4")
-    return out
 
 
 MX4_FEW_ROWS = 64              # up to this many rows a product is one launch that quantises them itself
@@ -2121,114 +2103,95 @@ def mx4_row_splits(tiles: int, k: int, n_sm: int = 148) -> int:
     return s
 
 
-def _mx4_few(x) -> bool:
-    return (x.shape[0] <= MX4_FEW_ROWS and x.data_ptr() % 16 == 0
-            and (x.shape[0] == 1 or x.stride(0) * x.element_size() % 16 == 0))
-
-
-def _gemm_mx4_rows(x, w, out, n, epilogue, glu=None, splits=None):
-    limit, alpha, shift = glu or (0.0, 1.0, 0.0)
-    m, k = x.shape
-    if splits is None:
-        splits = mx4_row_splits(-(-n // 128), k, sm_count(x.device))
-    st = _lib("mx4_rows").rllm_gemm_mx4_rows(
-        _ptr(x), c_int(_code(x)), c_longlong(x.stride(0) if m > 1 else 0), _ptr(w.codes), _ptr(w.scales), _ptr(out), c_int(_code(out)),
-        c_longlong(out.stride(0) if m > 1 else n), c_int(m), c_int(n), c_int(k), c_int(epilogue), c_int(splits), c_int(1 if w.settled else 0), c_float(limit),
-        c_float(alpha), c_float(shift), _ptr(error_word(x.device)), _stream())
+def _mx4_product(x, w, out, lead, epilogue, glu, who, splits=None, offsets=None, place=None, top_k=0):
+    """Checks and launches: x [m, k] (the rows before they are sorted, with `place`), w a stack `lead` of [n, k], out [rows, n].
+    A launch for up to 64 rows that lie as the kernel reads them; else one that quantises the rows into a workspace and one that
+    multiplies."""
+    _need_cuda(x, w, out)
+    _mx4_current(x, w, out)
+    m, k, ldx = _mx4_rows(x, who)
+    if out.dim() != 2:
+        raise KernelError(f"{who}: an output of {out.dim()} dimensions")
+    rows, n = out.shape
+    if w.shape != (*lead, n, k):
+        raise KernelError(f"{who}: a weight {w.shape} where {(*lead, n, k)} is needed")
+    ldc = out.stride(0) if rows > 1 else n
+    if (n > 1 and out.stride(1) != 1) or ldc < n:
+        raise KernelError(f"{who}: an output with strides {out.stride()} for {n} columns")
+    if rows != (m if place is None else m * top_k):
+        raise KernelError(f"{who}: an output of {rows} rows for {m} rows" + (f" and {top_k} experts each" if place is not None else ""))
+    x_code, out_code = _code(x), _code(out)
+    if epilogue == EPI_ACCUM and out_code != F32:
+        raise KernelError("accumulating product needs a float32 output")
+    if rows == 0 or n == 0:
+        return out
+    err, ahead = error_word(x.device), 1 if w.settled else 0
+    if offsets is None and m <= MX4_FEW_ROWS and x.data_ptr() % 16 == 0 and (m == 1 or ldx * x.element_size() % 16 == 0):
+        if splits is None:
+            splits = mx4_row_splits(-(-n // 128), k, sm_count(x.device))
+        st = _mx4_few((x, w.codes, w.scales, out, err), (ldx if m > 1 else 0, ldc, x_code, out_code, m, n, k, epilogue, splits, ahead), glu)
+    else:
+        experts = lead[0] if offsets is not None else 1
+        blocks = -(-rows // 128) + (experts if offsets is not None else 0)
+        work = torch.empty((rows * (k // 2) + 1023 & -1024) + blocks * -(-k // 256) * 1024, dtype=torch.uint8, device=x.device)
+        st = _mx4_many((x, offsets, place, w.codes, w.scales, out, work, err),
+                       (ldx, ldc, x_code, out_code, rows, n, k, experts, top_k, epilogue, ahead), glu)
+        add_launches(1)
     if st >= 30000:
-        raise KernelError(f"gemm_mx4_rows: tensor map encoding failed (CUresult {st - 30000})")
-    _check(st, "gemm_mx4_rows")
+        raise KernelError(f"{who}: tensor map encoding failed (CUresult {st - 30000})")
+    _check(st, who)
     return out
 
 
-def _mx4_product(x, w, out, n, lead, who):
-    """Checks that the products have in common: x [m, k], w a stack `lead` of [n, k], out [m, n]."""
-    _need_cuda(x, w, out)
-    _mx4_current(x, w, out)
-    _mx4_rows(x, who)
-    if tuple(w.shape) != tuple(lead) + (n, x.shape[1]):
-        raise KernelError(f"{who}: a weight {tuple(w.shape)} where {tuple(lead) + (n, x.shape[1])} is needed")
-    if out.dim() != 2 or out.shape[1] != n or (n > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < n):
-        raise KernelError(f"{who}: an output {tuple(out.shape)} with strides {out.stride()} for {n} columns")
+_SWIGLU = (0.0, 1.0, 0.0)
 
 
 def mx4_linear(x, w, out=None, out_dtype=None, accumulate=False):
     """out [m, n] (+)= Q(x) W^T: the rows x [m, k] (float32 or bfloat16) become 4-bit numbers as by `mx4_quantize`, w [n, k] is an
     Mx4Matrix; products of 4-bit numbers with float32 sums.  accumulate: `out` is float32 and the product is added to it."""
-    m, n = x.shape[0], w.shape[0]
     if out is None:
         if accumulate:
             raise KernelError("mx4_linear: accumulate needs an output to add to")
-        out = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
-    _mx4_product(x, w, out, n, (), "mx4_linear")
-    if out.shape[0] != m:
-        raise KernelError(f"mx4_linear: an output of {out.shape[0]} rows for {m}")
-    if accumulate and out.dtype != torch.float32:
-        raise KernelError("accumulating product needs a float32 output")
-    if m and n:
-        epilogue = EPI_ACCUM if accumulate else EPI_STORE
-        if _mx4_few(x):
-            return _gemm_mx4_rows(x, w, out, n, epilogue)
-        _gemm_mx4(*_mx4_operand(x, "mx4_linear"), w, out, n, epilogue)
-    return out
+        out = torch.empty((x.shape[0], w.shape[-2]), dtype=out_dtype or x.dtype, device=x.device)
+    return _mx4_product(x, w, out, (), EPI_ACCUM if accumulate else EPI_STORE, _SWIGLU, "mx4_linear")
 
 
 def mx4_gated(h, w, out, glu=None):
     """out [m, F] = glu(Q(h) Wg^T, Q(h) Wu^T), w the stack [2, F, k] of gate and up; glu = (limit, alpha, shift) as for
     gate_up_swiglu (None: SwiGLU)."""
-    m, F = out.shape
-    _mx4_product(h, w, out, F, (2,), "mx4_gated")
-    if h.shape[0] != m:
-        raise KernelError(f"mx4_gated: an output of {m} rows for {h.shape[0]}")
-    if m and F:
-        if _mx4_few(h):
-            return _gemm_mx4_rows(h, w, out, F, EPI_SWIGLU, glu)
-        _gemm_mx4(*_mx4_operand(h, "mx4_gated"), w, out, F, EPI_SWIGLU, glu)
-    return out
+    return _mx4_product(h, w, out, (2,), EPI_SWIGLU, glu or _SWIGLU, "mx4_gated")
 
 
-def _mx4_sorted(x, rows, offsets, place, experts, who):
-    """The sorted rows of routed experts as an operand: x the tokens' rows with `place`, or the sorted rows themselves."""
-    k = x.shape[1]
+def _mx4_experts(experts, rows, offsets, place, who):
     if not 0 < experts <= MX4_MAX_EXPERTS:
         raise KernelError(f"{who}: {experts} experts (1 to {MX4_MAX_EXPERTS})")
     for name, t, size in (("offsets", offsets, experts + 1), ("place", place, rows)):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != size):
-            raise KernelError(f"{who}: {name} is int32 [{size}]")
-    _need_cuda(offsets, place)
-    _mx4_current(offsets, place)
-    codes = torch.empty((rows, k // 2), dtype=torch.uint8, device=x.device)
-    # every expert's rows begin a block of 128 scale rows
-    scales = torch.empty((-(-rows // 128) + experts,) + mx4_scale_shape(1, k)[1:], dtype=torch.uint8, device=x.device)
-    _mx4_quantize(x, codes, scales, 0, offsets, place, experts, rows // x.shape[0] if place is not None else 0)
-    return codes, scales
+        if t is not None:
+            _need_cuda(t)
+            _mx4_current(t)
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != size:
+                raise KernelError(f"{who}: {name} is int32 [{size}]")
 
 
 def mx4_experts_up(h, w, offsets, place, act, glu=None):
     """The gated product of routed experts: act[place[p]] = glu(Q(h[p // top_k]) Wg[e]^T, Q(h[p // top_k]) Wu[e]^T) for the pairs p of
     h [n, d] with their experts e, sorted by `moe_sort` (offsets [E + 1], place [n * top_k]); w [E, 2, F, d] as an Mx4Matrix, act
     [n * top_k, F].  Two launches, whatever the experts' counts; no host involvement."""
-    pairs, F = act.shape
-    if len(w.shape) != 4 or h.dim() != 2 or (h.shape[0] and pairs % h.shape[0]) or (pairs and not h.shape[0]):
-        raise KernelError(f"mx4_experts_up: {pairs} pairs of {tuple(h.shape)} rows, weights {tuple(w.shape)}")
-    E = w.shape[0]
-    _mx4_product(h, w, act, F, (E, 2), "mx4_experts_up")
-    if pairs and F:
-        _gemm_mx4(*_mx4_sorted(h, pairs, offsets, place, E, "mx4_experts_up"), w, act, F, EPI_SWIGLU, glu, offsets, E)
-    return act
+    pairs, n = act.shape[0], h.shape[0]
+    if len(w.shape) != 4:
+        raise KernelError(f"mx4_experts_up: weights {w.shape} where [E, 2, F, d] is needed")
+    _mx4_experts(w.shape[0], pairs, offsets, place, "mx4_experts_up")
+    return _mx4_product(h, w, act, (w.shape[0], 2), EPI_SWIGLU, glu or _SWIGLU, "mx4_experts_up", None, offsets, place,
+                        pairs // n if n else 0)
 
 
 def mx4_experts_down(act, w, offsets, y):
     """The experts' second product: y[r] = Q(act[r]) W[e]^T for the sorted rows r of expert e (offsets [E + 1]); w [E, n, k] as an
     Mx4Matrix, y [rows, n] float32 or bfloat16.  `moe_combine` adds a token's rows up with the router's weights."""
-    rows, n = y.shape
-    if len(w.shape) != 3 or act.dim() != 2 or act.shape[0] != rows:
-        raise KernelError(f"mx4_experts_down: {tuple(act.shape)} rows, weights {tuple(w.shape)}, output {tuple(y.shape)}")
-    E = w.shape[0]
-    _mx4_product(act, w, y, n, (E,), "mx4_experts_down")
-    if rows and n:
-        _gemm_mx4(*_mx4_sorted(act, rows, offsets, None, E, "mx4_experts_down"), w, y, n, EPI_STORE, None, offsets, E)
-    return y
+    if len(w.shape) != 3:
+        raise KernelError(f"mx4_experts_down: weights {w.shape} where [E, n, k] is needed")
+    _mx4_experts(w.shape[0], 0, offsets, None, "mx4_experts_down")
+    return _mx4_product(act, w, y, (w.shape[0],), EPI_STORE, _SWIGLU, "mx4_experts_down", None, offsets)
 
 
 FLASH_HEAD_DIMS = (64, 128)

@@ -390,15 +390,15 @@ def test_few_rows_shared_k(m, n, k, splits):
         want, size = plain.product(xq, values)
         slack = plain.product_slack(size, k)
         out = torch.full((m + 1, n + 2), 5.0, device=DEV)
-        o._gemm_mx4_rows(x, w, out[:m, :n], n, o.EPI_STORE, splits=splits)
+        o._mx4_product(x, w, out[:m, :n], (), o.EPI_STORE, SWIGLU, "", splits)
         plain.near(out[:m, :n], want, slack)
         c = rnd(m, n, seed=4)
         out[:m, :n] = c
-        o._gemm_mx4_rows(x, w, out[:m, :n], n, o.EPI_ACCUM, splits=splits)
+        o._mx4_product(x, w, out[:m, :n], (), o.EPI_ACCUM, SWIGLU, "", splits)
         plain.near(out[:m, :n], want + c.double(), slack + 2.0 ** -24 * (want.abs() + c.double().abs()))
         out[:m, :n] = 5.0
         assert bool((out == 5.0).all())
         act = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
-        o._gemm_mx4_rows(x, g, act, n, o.EPI_SWIGLU, glu=CLAMPED, splits=splits)
+        o._mx4_product(x, g, act, (2,), o.EPI_SWIGLU, CLAMPED, "", splits)
         plain.near(act, *plain.gated(xq, gv[0], gv[1], CLAMPED))
     o.check_device_errors()
