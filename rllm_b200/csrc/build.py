@@ -45,7 +45,7 @@ LIBRARIES = {
     "group": (["gemm_group.cu"], []),
     "stream": (["gemv_stream.cu"], []),
     "mx4": (["mx4.cu", "gemm_mx4.cu"], []),
-    "mx4_rows": (["gemm_mx4_rows.cu"], []),
+    "mx4_rows": (["gemm_mx4_rows.cu", "mx4.cu"], []),
     "attn_tc": (["attention_tc.cu"], []),
     "host": (["host_runtime.cpp"], []),
 }

@@ -2047,7 +2047,7 @@ def mx4_scale_shape(n: int, k: int) -> tuple:
 _mx4_quantize = _Packed("mx4", "rllm_mx4_quantize", 5, 7)
 _mx4_dequantize = _Packed("mx4", "rllm_mx4_dequantize", 3, 4)
 _mx4_many = _Packed("mx4", "rllm_mx4_product", 8, 11, 3)
-_mx4_few = _Packed("mx4_rows", "rllm_gemm_mx4_rows", 5, 10, 3)
+_mx4_few = _Packed("mx4_rows", "rllm_mx4_rows_product", 8, 13, 3)
 
 
 def _mx4_current(*ts):
@@ -2092,21 +2092,37 @@ def mx4_quantize(x):
     return Mx4Matrix(codes, scales)
 
 
-MX4_FEW_ROWS = 64              # up to this many rows a product is one launch that quantises them itself
+MX4_OWN_ROWS = 16              # up to this many rows a product is one launch that quantises them itself,
+MX4_OWN_PAIRS = 256            # and up to this many pairs of tokens and experts
 
 
-def mx4_row_splits(tiles: int, k: int, n_sm: int = 148) -> int:
-    """CTAs that share the K of a tile of 128 weight rows in the product of few rows."""
-    chunks, s = -(-k // 256), 1
-    while s < 8 and 2 * s <= chunks and tiles * 2 * s <= 2 * n_sm:
+def mx4_row_splits(tiles: int, k: int, bn: int, gated: bool, n_sm: int = 148) -> int:
+    """CTAs that share the K of a tile of 128 weight rows in the product of few rows (tiles: with gate and up, experts and chunks of rows
+    counted apart): as many as all run at once, three an SM with up to 32 rows, else two."""
+    most, chunks, s = (3 if bn <= 32 else 2) * n_sm, -(-k // 256), 1
+    while s < (4 if gated else 8) and 2 * s <= chunks and tiles * 2 * s <= most:
         s *= 2
     return s
 
 
-def _mx4_product(x, w, out, lead, epilogue, glu, who, splits=None, offsets=None, place=None, top_k=0):
+def mx4_few_rows(rows: int, n: int, k: int, gated: bool, own: bool, experts: int = 0, n_sm: int = 148):
+    """(rows of x to a CTA, CTAs that share K) for the product of few rows (gemm_mx4_rows.cu), or None: the one of many rows
+    (gemm_mx4.cu).  own: the rows lie as the kernel that quantises them itself reads them; experts: of sorted rows (0: none)."""
+    tiles = -(-n // 128) * (2 if gated else 1)
+    if own and (rows <= MX4_OWN_PAIRS if experts else rows <= MX4_OWN_ROWS):
+        return 16, mx4_row_splits(tiles * min(experts, rows) if experts else tiles, k, 16, gated, n_sm)
+    if experts or rows > MX4_FEW_ROWS:
+        return None
+    bn = 32 if rows <= 32 else 64 if rows <= 64 else 128
+    return bn, mx4_row_splits(tiles * -(-rows // bn), k, bn, gated, n_sm)
+
+
+MX4_FEW_ROWS = 64
+
+
+def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, place=None, top_k=0):
     """Checks and launches: x [m, k] (the rows before they are sorted, with `place`), w a stack `lead` of [n, k], out [rows, n].
-    A launch for up to 64 rows that lie as the kernel reads them; else one that quantises the rows into a workspace and one that
-    multiplies."""
+    few: as mx4_few_rows answers (False for None), by default what it answers."""
     _need_cuda(x, w, out)
     _mx4_current(x, w, out)
     m, k, ldx = _mx4_rows(x, who)
@@ -2126,17 +2142,20 @@ def _mx4_product(x, w, out, lead, epilogue, glu, who, splits=None, offsets=None,
     if rows == 0 or n == 0:
         return out
     err, ahead = error_word(x.device), 1 if w.settled else 0
-    if offsets is None and m <= MX4_FEW_ROWS and x.data_ptr() % 16 == 0 and (m == 1 or ldx * x.element_size() % 16 == 0):
-        if splits is None:
-            splits = mx4_row_splits(-(-n // 128), k, sm_count(x.device))
-        st = _mx4_few((x, w.codes, w.scales, out, err), (ldx if m > 1 else 0, ldc, x_code, out_code, m, n, k, epilogue, splits, ahead), glu)
-    else:
-        experts = lead[0] if offsets is not None else 1
-        blocks = -(-rows // 128) + (experts if offsets is not None else 0)
-        work = torch.empty((rows * (k // 2) + 1023 & -1024) + blocks * -(-k // 256) * 1024, dtype=torch.uint8, device=x.device)
-        st = _mx4_many((x, offsets, place, w.codes, w.scales, out, work, err),
-                       (ldx, ldc, x_code, out_code, rows, n, k, experts, top_k, epilogue, ahead), glu)
+    experts = lead[0] if offsets is not None else 0
+    if few is None:
+        own = x.data_ptr() % 16 == 0 and (m == 1 or ldx * x.element_size() % 16 == 0)
+        few = mx4_few_rows(rows, n, k, epilogue == EPI_SWIGLU, own, experts, sm_count(x.device))
+    work = None
+    if not few or few[0] != 16:
+        work = torch.empty((rows * (k // 2) + 1023 & -1024) + (-(-rows // 128) + experts) * -(-k // 256) * 1024, dtype=torch.uint8,
+                           device=x.device)
         add_launches(1)
+    tensors = (x, offsets, place, w.codes, w.scales, out, work, err)
+    if few:
+        st = _mx4_few(tensors, (ldx if m > 1 else 0, ldc, x_code, out_code, rows, n, k, experts, top_k, epilogue, *few, ahead), glu)
+    else:
+        st = _mx4_many(tensors, (ldx, ldc, x_code, out_code, rows, n, k, experts or 1, top_k, epilogue, ahead), glu)
     if st >= 30000:
         raise KernelError(f"{who}: tensor map encoding failed (CUresult {st - 30000})")
     _check(st, who)

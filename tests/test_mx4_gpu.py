@@ -173,7 +173,7 @@ def test_gated(m, F, k, form):
 
 # ---------------------------------------------------------------- routed experts
 
-ROUTES = [(1, 1, 1, 0), (1, 4, 2, 0), (5, 7, 3, 1), (40, 16, 4, 2), (64, 3, 2, 0), (200, 16, 4, 1), (301, 5, 5, 0), (130, 64, 1, 1)]
+ROUTES = [(1, 1, 1, 0), (1, 4, 2, 0), (64, 4, 4, 2), (17, 40, 8, 1), (5, 7, 3, 1), (40, 16, 4, 2), (64, 3, 2, 0), (200, 16, 4, 1), (301, 5, 5, 0), (130, 64, 1, 1)]
 
 
 def route(n, E, top, skew, seed):
@@ -377,11 +377,15 @@ def test_offsets_that_do_not_rise():
 
 
 @pytest.mark.parametrize("splits", [1, 2, 4, 8])
-@pytest.mark.parametrize("m", [1, 2, 7, 16, 17, 40, 64])
+@pytest.mark.parametrize("m,bn", [(1, 16), (2, 16), (7, 16), (16, 16), (1, 32), (17, 32), (32, 32), (40, 64), (64, 64), (90, 128), (128, 128),
+                                  (300, 128), (70, 0)])
 @pytest.mark.parametrize("n,k", [(200, 2080), (128, 256), (1000, 8192)])
-def test_few_rows_shared_k(m, n, k, splits):
-    """Every way to share K, also between more CTAs than there are chunks of K; float32 rows; a ring that wraps."""
+def test_few_rows_shared_k(m, bn, n, k, splits):
+    """Every kernel for few rows with every way to share K; float32 rows; a ring that wraps.  bn 0: the kernel for many rows."""
     o = ops()
+    if splits > -(-k // 256) or (not bn and splits > 1):
+        pytest.skip("fewer chunks of K than CTAs")
+    few, few_gated = ((bn, splits), (bn, min(splits, 4))) if bn else (False, False)
     w, values = weight(n, k, seed=1)
     g, gv = weight(2, n, k, seed=2)
     for dtype in (torch.bfloat16, torch.float32):
@@ -390,15 +394,16 @@ def test_few_rows_shared_k(m, n, k, splits):
         want, size = plain.product(xq, values)
         slack = plain.product_slack(size, k)
         out = torch.full((m + 1, n + 2), 5.0, device=DEV)
-        o._mx4_product(x, w, out[:m, :n], (), o.EPI_STORE, SWIGLU, "", splits)
+        o._mx4_product(x, w, out[:m, :n], (), o.EPI_STORE, SWIGLU, "", few)
         plain.near(out[:m, :n], want, slack)
         c = rnd(m, n, seed=4)
         out[:m, :n] = c
-        o._mx4_product(x, w, out[:m, :n], (), o.EPI_ACCUM, SWIGLU, "", splits)
+        o._mx4_product(x, w, out[:m, :n], (), o.EPI_ACCUM, SWIGLU, "", few)
         plain.near(out[:m, :n], want + c.double(), slack + 2.0 ** -24 * (want.abs() + c.double().abs()))
         out[:m, :n] = 5.0
         assert bool((out == 5.0).all())
         act = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
-        o._mx4_product(x, g, act, (2,), o.EPI_SWIGLU, CLAMPED, "", splits)
+        g.settled = True
+        o._mx4_product(x, g, act, (2,), o.EPI_SWIGLU, CLAMPED, "", few_gated)
         plain.near(act, *plain.gated(xq, gv[0], gv[1], CLAMPED))
     o.check_device_errors()
