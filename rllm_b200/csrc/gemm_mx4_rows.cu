@@ -72,7 +72,7 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
     __shared__ int s_src[BN];
     float* red = reinterpret_cast<float*>(smem);             // parked sums [row of X][weight row]: the stages are free by then
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int ranks = gridDim.y, n_splits = ranks / HALVES, half = (int)blockIdx.y / n_splits, split = (int)blockIdx.y - half * n_splits;
     const int n0 = blockIdx.x * 128;
     const int nkb = (K + MX4_CHUNK - 1) / MX4_CHUNK;
@@ -130,75 +130,78 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = tmem_base_slot;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
     float v[COLS];                                           // the epilogue threads' accumulator rows
     bool ep_ok = true;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
         // ---- the weights and their scales, and the rows' where they come as codes.  Settled weights fill the ring ahead of the wait
+        const uint32_t on = warp_elect(), ring = s_addr(smem);
         const long long g = (long long)e * HALVES + half;
-        const uint8_t* sf = sfw + (size_t)(g * ((n + 127) >> 7) + blockIdx.x) * rb_bytes;
-        auto load_w = [&](int i) {
-            const int s = i % STAGES;
-            unsigned char* w_s = smem + (size_t)s * STAGE_BYTES;
-            mbar_expect_tx(&full_bar[s], TX_BYTES);
-            tma_load_2d(w_s, &tmW, (kb0 + i) * 128, (int)(g * n) + n0, &full_bar[s]);
-            bulk_load(w_s + W_BYTES + X_BYTES, sf + (size_t)(kb0 + i) * MX4_SF_BYTES, MX4_SF_BYTES, &full_bar[s]);
+        const uint8_t* sf = sfw + (size_t)(g * ((n + 127) >> 7) + blockIdx.x) * rb_bytes + (size_t)kb0 * MX4_SF_BYTES;
+        auto load_w = [&](int s, int i) {
+            const uint32_t w_s = ring + s * STAGE_BYTES;
+            warp_expect_tx(on, &full_bar[s], TX_BYTES);
+            warp_load_2d(on, w_s, &tmW, (kb0 + i) * 128, (int)(g * n) + n0, &full_bar[s]);
+            warp_bulk_load(on, w_s + W_BYTES + X_BYTES, sf + (size_t)i * MX4_SF_BYTES, MX4_SF_BYTES, &full_bar[s]);
         };
         const int head = ahead && !so.offsets ? min(STAGES, my_kb) : 0;
-        for (int i = 0; i < head; ++i) load_w(i);
+        for (int i = 0; i < head; ++i) load_w(i, i);
         if (!so.offsets) pdl_wait();
-        int issued = head;
+        int issued = head, s = 0;
+        uint32_t ph = 1;
         for (int i = 0; i < my_kb; ++i) {
-            const int s = i % STAGES;
             if (i >= head) {
-                if (!mbar_wait(&empty_bar[s], ((i / STAGES) & 1) ^ 1, &abort_flag)) {
+                if (!warp_wait(&empty_bar[s], ph, &abort_flag)) {
                     if (!abort_flag) { atomicExch(err, GR_ERR_EMPTY); abort_flag = 1; }
                     break;
                 }
-                load_w(i);
+                load_w(s, i);
                 issued = i + 1;
             }
             if (CODES) {
-                unsigned char* x_s = smem + (size_t)s * STAGE_BYTES + W_BYTES;
-                tma_load_2d(x_s, &tmX, (kb0 + i) * 128, r0, &full_bar[s]);
-                bulk_load(x_s + X_BYTES + MX4_SF_BYTES,
-                          reinterpret_cast<const uint8_t*>(X) + (size_t)(r0 >> 7) * rb_bytes + (size_t)(kb0 + i) * MX4_SF_BYTES, MX4_SF_BYTES,
-                          &full_bar[s]);
+                const uint32_t x_s = ring + s * STAGE_BYTES + W_BYTES;
+                warp_load_2d(on, x_s, &tmX, (kb0 + i) * 128, r0, &full_bar[s]);
+                warp_bulk_load(on, x_s + X_BYTES + MX4_SF_BYTES,
+                               reinterpret_cast<const uint8_t*>(X) + (size_t)(r0 >> 7) * rb_bytes + (size_t)(kb0 + i) * MX4_SF_BYTES, MX4_SF_BYTES,
+                               &full_bar[s]);
             }
+            if (++s == STAGES) { s = 0; ph ^= 1; }
         }
         if (abort_flag) {
             // copies already issued must land before the CTA's shared memory goes away
             volatile int no_abort = 0;
             for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1, &no_abort);
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         // ---- issuer
+        const uint32_t on = warp_elect(), ring = s_addr(smem);
+        const uint32_t w0 = tile_lo(ring), x0 = tile_lo(ring + W_BYTES), f0 = atom_lo(ring + W_BYTES + X_BYTES);
+        int s = 0;
+        uint32_t ph = 0;
         bool ok = true;
         for (int i = 0; i < my_kb; ++i) {
-            const int s = i % STAGES;
-            if (!mbar_wait(&full_bar[s], (i / STAGES) & 1, &abort_flag) ||
-                (!CODES && !mbar_wait(&rows_bar[s], (i / STAGES) & 1, &abort_flag))) {
+            if (!warp_wait(&full_bar[s], ph, &abort_flag) || (!CODES && !warp_wait(&rows_bar[s], ph, &abort_flag))) {
                 if (!abort_flag) { atomicExch(err, GR_ERR_FULL); abort_flag = 1; }
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t w_addr = s_addr(smem + (size_t)s * STAGE_BYTES), x_addr = w_addr + W_BYTES, f_addr = x_addr + X_BYTES;
+            const uint32_t at = s * (STAGE_BYTES >> 4), f = f0 + at;
             const uint32_t t_w = tmem_base + BN + s * SF_COLS, t_x = t_w + 8;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                tmem_cp_atom(t_w + 4 * g, smem_desc_atom(f_addr + g * MX4_ATOM));
-                tmem_cp_atom(t_x + 4 * g, smem_desc_atom(f_addr + MX4_SF_BYTES + g * MX4_ATOM));
+                tmem_cp_atom<1>(on, t_w + 4 * g, atom_desc(f + g * (MX4_ATOM >> 4)));
+                tmem_cp_atom<1>(on, t_x + 4 * g, atom_desc(f + (MX4_SF_BYTES >> 4) + g * (MX4_ATOM >> 4)));
             }
-            const uint64_t w_desc = smem_desc_sw128(w_addr), x_desc = smem_desc_sw128(x_addr);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-                umma_mxf4(tmem_base, w_desc + 2 * kk, x_desc + 2 * kk, idesc_mxf4(128, BN, (kk & 1) * 2), t_w + 4 * (kk >> 1),
-                          t_x + 4 * (kk >> 1), (i | kk) != 0);
-            umma_commit(&empty_bar[s]);
+                umma_mxf4<1>(on, tmem_base, tile_desc(w0 + at + 2 * kk), tile_desc(x0 + at + 2 * kk), idesc_mxf4(128, BN, (kk & 1) * 2),
+                             t_w + 4 * (kk >> 1), t_x + 4 * (kk >> 1), (i | kk) != 0);
+            umma_done<1>(on, &empty_bar[s]);
+            if (++s == STAGES) { s = 0; ph ^= 1; }
         }
-        if (ok) umma_commit(&acc_bar);
+        if (ok) umma_done<1>(on, &acc_bar);
     } else if (warp >= 2) {
         // ---- first the rows of X into the stages: warp w takes rows w, w + QW, ... of every stage
         if (!so.offsets) pdl_wait();

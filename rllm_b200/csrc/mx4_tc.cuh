@@ -7,27 +7,89 @@
 #define MX4_SF_BYTES (2 * MX4_ATOM)                        // the scales of 128 rows in a stage of 256 entries along K
 
 // ---------------------------------------------------------------- the instructions
+// A role's whole warp runs its loop and one elected lane issues (the predicate `on` of the wrappers below): the loop's counters and addresses
+// are then uniform over the warp and live in uniform registers, which is where these instructions take their operands from.  With the
+// loop inside `if (lane == 0)` every operand is moved there first, and the eleven instructions of a stage took about 1,000 cycles to issue.
+__device__ __forceinline__ uint32_t warp_elect() {
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+    return on;
+}
+// mbar_wait by a whole warp with one answer
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
 // Instruction descriptor of kind mxf4: A and B e2m1 (1), scales ue8m0 (bit 23), both operands K-major, shape M x N x 64; bits 4-5 and
 // 29-30 say which bytes of the scale columns belong to B and A (0 or 2: two scales a row and instruction).
 __host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, int sf_id) {
     return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | ((uint32_t)sf_id << 4) |
            ((uint32_t)sf_id << 29);
 }
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                          uint32_t accumulate) {
+// Descriptors by their low words (upper words are constant): a K-major tile with 128-byte swizzle (smem_desc_sw128), and one atom of scales,
+// 32 lines of 16 bytes without swizzle, groups of 8 lines 128 bytes apart.  Shared memory ends below 2^18, so an offset in 16-byte units may be
+// added to a low word.
+__device__ __forceinline__ uint32_t tile_lo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t atom_lo(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4; }
+__device__ __forceinline__ uint64_t tile_desc(uint32_t lo) { return ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32) | lo; }
+__device__ __forceinline__ uint64_t atom_desc(uint32_t lo) { return ((uint64_t)((128u >> 4) | (1u << 14)) << 32) | lo; }
+
+// CG: CTAs that work together (the instructions' cta_group)
+template <int CG> __device__ __forceinline__ void umma_mxf4(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(on) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(on) : "memory");
+}
+// 512 bytes -> four columns, the 32 lines repeated for the four quarters of the lanes (CG 2: in each CTA its own bytes)
+template <int CG> __device__ __forceinline__ void tmem_cp_atom(uint32_t on, uint32_t taddr, uint64_t desc) {
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}"
+                     ::"r"(taddr), "l"(desc), "r"(on) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}"
+                     ::"r"(taddr), "l"(desc), "r"(on) : "memory");
+}
+// CG 2: arrives at the barrier at this offset in both CTAs
+template <int CG> __device__ __forceinline__ void umma_done(uint32_t on, uint64_t* bar) {
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                     ::"r"(s_addr(bar)), "r"(on) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}"
+                     ::"r"(s_addr(bar)), "r"(on), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void warp_expect_tx(uint32_t on, uint64_t* bar, uint32_t bytes) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+                 ::"r"(s_addr(bar)), "r"(bytes), "r"(on) : "memory");
+}
+__device__ __forceinline__ void warp_load_2d(uint32_t on, uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+        ::"r"(dst), "l"(map), "r"(s_addr(bar)), "r"(x), "r"(y), "r"(on) : "memory");
 }
-// Shared-memory descriptor of one atom of scales: 32 lines of 16 bytes without swizzle, groups of 8 lines 128 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_atom(uint32_t saddr) {
-    return ((uint64_t)((128u >> 4) | (1u << 14)) << 32) | ((saddr & 0x3FFFFu) >> 4);
+// the bytes complete on a barrier given by its cluster address (the leader's)
+__device__ __forceinline__ void warp_load_2d_pair(uint32_t on, uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(on) : "memory");
 }
-// 512 bytes -> four columns, the 32 lines repeated for the four quarters of the lanes
-__device__ __forceinline__ void tmem_cp_atom(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void warp_bulk_load(uint32_t on, uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+                 "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(s_addr(bar)), "r"(on) : "memory");
 }
 // 8 and 16 columns of the warp's lanes
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* r) {
@@ -41,14 +103,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* r) {
           "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
         : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(s_addr(dst)), "l"(src), "r"(bytes), "r"(s_addr(bar)) : "memory");
-}
 
 // ---------------------------------------------------------------- host side
 // Tensor map of codes [rows, k / 2] (contiguous): boxes of box_rows x 128 bytes, 128-byte swizzle, zeros outside.
-static int mx4_tmap(CUtensorMap* map, const void* base, long long rows, int k, int box_rows) {
+static inline int mx4_tmap(CUtensorMap* map, const void* base, long long rows, int k, int box_rows) {
     TmapEncodeFn enc = tmap_encoder();
     if (!enc) return 30001;
     const cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)rows};
@@ -56,6 +114,19 @@ static int mx4_tmap(CUtensorMap* map, const void* base, long long rows, int k, i
     const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, estr[2] = {1, 1};
     const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : 30000 + (int)r;
+}
+
+// Tensor map of scales: `lines` of 1,024 bytes (128 rows by 256 entries along K each), a line a box.
+static inline int mx4_scale_tmap(CUtensorMap* map, const void* base, long long lines) {
+    TmapEncodeFn enc = tmap_encoder();
+    if (!enc) return 30001;
+    const cuuint64_t dims[2] = {256, (cuuint64_t)lines};
+    const cuuint64_t strides[1] = {MX4_SF_BYTES};
+    const cuuint32_t box[2] = {256, 1}, estr[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : 30000 + (int)r;
 }

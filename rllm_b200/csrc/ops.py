@@ -2046,7 +2046,7 @@ def mx4_scale_shape(n: int, k: int) -> tuple:
 
 _mx4_quantize = _Packed("mx4", "rllm_mx4_quantize", 5, 7)
 _mx4_dequantize = _Packed("mx4", "rllm_mx4_dequantize", 3, 4)
-_mx4_many = _Packed("mx4", "rllm_mx4_product", 8, 11, 3)
+_mx4_many = _Packed("mx4", "rllm_mx4_product", 8, 12, 3)
 _mx4_few = _Packed("mx4_rows", "rllm_mx4_rows_product", 8, 13, 3)
 
 
@@ -2120,7 +2120,12 @@ def mx4_few_rows(rows: int, n: int, k: int, gated: bool, own: bool, experts: int
 MX4_FEW_ROWS = 64
 
 
-def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, place=None, top_k=0):
+def mx4_pairs(rows: int, n: int, gated: bool, experts: int = 0, n_sm: int = 148) -> bool:
+    """Whether the product of many rows takes two SMs to a tile of 256 x 256, or one to a tile of 128 x 256."""
+    return rows > 128 * max(1, experts)
+
+
+def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, place=None, top_k=0, pairs=None):
     """Checks and launches: x [m, k] (the rows before they are sorted, with `place`), w a stack `lead` of [n, k], out [rows, n].
     few: as mx4_few_rows answers (False for None), by default what it answers."""
     _need_cuda(x, w, out)
@@ -2155,7 +2160,9 @@ def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, pl
     if few:
         st = _mx4_few(tensors, (ldx if m > 1 else 0, ldc, x_code, out_code, rows, n, k, experts, top_k, epilogue, *few, ahead), glu)
     else:
-        st = _mx4_many(tensors, (ldx, ldc, x_code, out_code, rows, n, k, experts or 1, top_k, epilogue, ahead), glu)
+        if pairs is None:
+            pairs = mx4_pairs(rows, n, epilogue == EPI_SWIGLU, experts, sm_count(x.device))
+        st = _mx4_many(tensors, (ldx, ldc, x_code, out_code, rows, n, k, experts or 1, top_k, epilogue, int(pairs), ahead), glu)
     if st >= 30000:
         raise KernelError(f"{who}: tensor map encoding failed (CUresult {st - 30000})")
     _check(st, who)

@@ -26,6 +26,15 @@ def weight(*shape, seed):
     return ops().Mx4Matrix.from_blocks(plain.pack(codes), scales.to(torch.uint8)), values
 
 
+@pytest.fixture(params=["by rule", "one SM a tile", "two SMs a tile"])
+def many(request, monkeypatch):
+    """The kernels that the sizes lead to; or those for many rows, whatever the sizes."""
+    if request.param != "by rule":
+        monkeypatch.setattr(ops(), "mx4_few_rows", lambda *a: None)
+        monkeypatch.setattr(ops(), "mx4_pairs", lambda *a: request.param.startswith("two"))
+    return request.param
+
+
 # ---------------------------------------------------------------- rows to codes and back
 
 def same(q, x):
@@ -95,7 +104,7 @@ SHAPES = [(1, 1, 32), (1, 128, 256), (2, 200, 64), (5, 130, 288), (8, 4096, 1024
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-def test_linear(m, n, k):
+def test_linear(m, n, k, many):
     x = rnd(m, k, seed=1, dtype=torch.bfloat16)
     w, values = weight(n, k, seed=2)
     want, size = plain.product(plain.quantize(x)[2], values)
@@ -113,7 +122,7 @@ def test_linear(m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(3, 40, 96), (70, 300, 288), (140, 130, 512)])
-def test_linear_strides_and_margins(m, n, k):
+def test_linear_strides_and_margins(m, n, k, many):
     """Rows of wider matrices in and out, at addresses that no 16 bytes divide; what lies beside the output stays."""
     w, values = weight(n, k, seed=2)
     for dtype in (torch.bfloat16, torch.float32):
@@ -129,7 +138,7 @@ def test_linear_strides_and_margins(m, n, k):
 
 
 @pytest.mark.parametrize("m", [2, 100])
-def test_linear_not_finite(m):
+def test_linear_not_finite(m, many):
     """A row with a NaN or an infinity gives a row of NaN, a weight's block that is not a number a column; nothing else changes."""
     n, k = 150, 320
     x = rnd(m, k, seed=1, dtype=torch.bfloat16)
@@ -143,7 +152,7 @@ def test_linear_not_finite(m):
 
 
 @pytest.mark.parametrize("m", [3, 130])
-def test_linear_scales_far_apart(m):
+def test_linear_scales_far_apart(m, many):
     """Scales from 2^-127 to 2^100: a block's power of two counts wherever it lies."""
     n, k = 140, 512
     g = torch.Generator().manual_seed(1)
@@ -157,7 +166,7 @@ def test_linear_scales_far_apart(m):
 
 @pytest.mark.parametrize("form", [None, CLAMPED, GELU])
 @pytest.mark.parametrize("m,F,k", [(1, 1, 32), (1, 96, 256), (8, 1536, 1024), (16, 130, 288), (40, 200, 2080), (65, 257, 544), (300, 1000, 512)])
-def test_gated(m, F, k, form):
+def test_gated(m, F, k, form, many):
     h = rnd(m, k, seed=1, dtype=torch.bfloat16)
     w, values = weight(2, F, k, seed=2)
     if form == CLAMPED:
@@ -186,7 +195,7 @@ def route(n, E, top, skew, seed):
 
 @pytest.mark.parametrize("n,E,top,skew", ROUTES)
 @pytest.mark.parametrize("d,F,form", [(256, 96, None), (288, 130, CLAMPED), (1024, 384, None)])
-def test_experts_up(n, E, top, skew, d, F, form):
+def test_experts_up(n, E, top, skew, d, F, form, many):
     idx, _ = route(n, E, top, skew, seed=n + E)
     h = rnd(n, d, seed=1, dtype=torch.bfloat16)
     w, values = weight(E, 2, F, d, seed=2)
@@ -205,7 +214,7 @@ def test_experts_up(n, E, top, skew, d, F, form):
 
 @pytest.mark.parametrize("n,E,top,skew", ROUTES)
 @pytest.mark.parametrize("F,d", [(96, 256), (160, 300), (384, 1024)])
-def test_experts_down(n, E, top, skew, F, d):
+def test_experts_down(n, E, top, skew, F, d, many):
     idx, wgt = route(n, E, top, skew, seed=n + E)
     offsets, place = ops().moe_sort(idx, E)
     act = rnd(n * top, F, seed=1, dtype=torch.bfloat16)
@@ -358,7 +367,7 @@ def test_refusals():
     o.mx4_experts_up(x[:0], e, offsets, place[:0], act[:0])
 
 
-def test_offsets_that_do_not_rise():
+def test_offsets_that_do_not_rise(many):
     """Offsets that are no offsets give rows without meaning, but no access outside the buffers."""
     o = ops()
     w, _ = weight(4, 2, 64, 128, seed=1)
