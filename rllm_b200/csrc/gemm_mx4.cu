@@ -22,7 +22,7 @@ RLLM_API int rllm_mx4_quantize(const void* x, void* codes, void* scales, const i
 
 #define GM_BM 128
 #define GM_BN 256
-#define GM_STAGES 4
+#define GM_STAGES 3
 #define GM_THREADS 320
 #define GM_MAX_E 1024
 #define GM_A_BYTES (GM_BM * 128)
@@ -32,31 +32,6 @@ RLLM_API int rllm_mx4_quantize(const void* x, void* codes, void* scales, const i
 
 enum { GM_EPI_STORE = 0, GM_EPI_ACCUM = 1, GM_EPI_GATED = 2 };
 enum { GM_ERR_FULL = 31, GM_ERR_EMPTY = 32, GM_ERR_ACC = 33 };
-
-template <typename TC> __device__ __forceinline__ void gm_store32(TC* dst, const float (&v)[32], int n_valid) {
-    if (n_valid >= 32 && ((uintptr_t)dst & 15) == 0) {
-        if constexpr (sizeof(TC) == 4) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t u[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * j + 2 * q], v[8 * j + 2 * q + 1]);
-                    u[q] = *reinterpret_cast<const uint32_t*>(&b);
-                }
-                reinterpret_cast<uint4*>(dst)[j] = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < n_valid) dst[j] = from_f<TC>(v[j]);
-    }
-}
 
 // A thread's half of an accumulator row into registers: 128 columns, gated 64 gate columns and the 64 up columns of the same index.
 template <bool GATED> __device__ __forceinline__ void gm_take(uint32_t taddr, int half, uint32_t (&r)[4][32]) {
@@ -71,32 +46,66 @@ template <bool GATED> __device__ __forceinline__ void gm_take(uint32_t taddr, in
     }
     tmem_ld_wait();
 }
-// ... and from there to the columns from n0 on of its row of C.
-template <typename TC, int EPI> __device__ __forceinline__ void gm_give(const uint32_t (&r)[4][32], TC* row, int n0, int N, const GluForm& glu) {
+// ... and from there to C.  A thread holds columns of one row; written as they are, 16 bytes a thread, a store would touch 32 lines, and the
+// stores of a tile of 128 x 256 float32 would take longer than its products at K 2,000.  So the warp's 32 rows pass through 4 KB of shared
+// memory, 128 bytes of each at a time (pieces of 16 bytes swizzled by the row), and leave as whole lines, eight lanes to a row.
+//   row0: the warp's first row, n0: the first column of what its threads hold, `vec`: rows of C begin at multiples of 16 bytes
+template <typename TC, int EPI> __device__ __forceinline__ void gm_give(const uint32_t (&r)[4][32], unsigned char* stage, int lane, TC* C, long long ldc,
+                                                                        int row0, int m_end, int n0, int N, bool vec, const GluForm& glu) {
     constexpr bool GATED = EPI == GM_EPI_GATED;
+    constexpr int PER = 128 / (int)sizeof(TC), PIECE = 16 / (int)sizeof(TC), OUT = GATED ? 64 : 128;
 #pragma unroll
-    for (int q = 0; q < (GATED ? 2 : 4); ++q) {
-        const int gn = n0 + q * 32;
-        if (gn >= N) break;
-        TC* dst = row + gn;
-        const int n_valid = min(32, N - gn);
-        float v[32];
+    for (int c = 0; c < OUT / PER; ++c) {
+        if (n0 + c * PER >= N) break;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            v[j] = GATED ? glu_apply(glu, __uint_as_float(r[q][j]), __uint_as_float(r[GATED ? q + 2 : q][j])) : __uint_as_float(r[q][j]);
-        if (EPI == GM_EPI_ACCUM) {
-            if (sizeof(TC) == 4 && n_valid >= 32 && ((uintptr_t)dst & 15) == 0) {
+        for (int j = 0; j < 8; ++j) {
+            float v[PIECE];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float4 c4 = reinterpret_cast<const float4*>(dst)[j];
-                    v[4 * j] += c4.x; v[4 * j + 1] += c4.y; v[4 * j + 2] += c4.z; v[4 * j + 3] += c4.w;
+            for (int i = 0; i < PIECE; ++i) {
+                const int col = c * PER + j * PIECE + i;
+                const float x = __uint_as_float(r[col >> 5][col & 31]);
+                v[i] = GATED ? mx4_glu(glu, x, __uint_as_float(r[(col >> 5) + (GATED ? 2 : 0)][col & 31])) : x;
+            }
+            uint4 u;
+            if constexpr (sizeof(TC) == 4) u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            else {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&b);
                 }
-            } else {
+                u = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+        }
+        __syncwarp();
+        const int col = n0 + c * PER + (lane & 7) * PIECE;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) if (j < n_valid) v[j] += to_f<TC>(dst[j]);
+        for (int i = 0; i < 8; ++i) {
+            const int row = i * 4 + (lane >> 3), gm = row0 + row;
+            uint4 u = *reinterpret_cast<const uint4*>(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+            if (gm < m_end && col < N) {
+                TC* dst = C + (size_t)gm * ldc + col;
+                if (vec && col + PIECE <= N) {
+                    if constexpr (EPI == GM_EPI_ACCUM) {
+                        const float4 o = *reinterpret_cast<const float4*>(dst);
+                        u = make_uint4(__float_as_uint(__uint_as_float(u.x) + o.x), __float_as_uint(__uint_as_float(u.y) + o.y),
+                                       __float_as_uint(__uint_as_float(u.z) + o.z), __float_as_uint(__uint_as_float(u.w) + o.w));
+                    }
+                    *reinterpret_cast<uint4*>(dst) = u;
+                } else {
+                    const TC* from = reinterpret_cast<const TC*>(&u);
+#pragma unroll
+                    for (int k = 0; k < PIECE; ++k)
+                        if (col + k < N) {
+                            if constexpr (EPI == GM_EPI_ACCUM) dst[k] += from[k];
+                            else dst[k] = from[k];
+                        }
+                }
             }
         }
-        gm_store32<TC>(dst, v, n_valid);
+        __syncwarp();
     }
 }
 
@@ -279,12 +288,13 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     } else if (warp >= 2) {
         // ---- epilogue: warp w may touch the lanes 32 * (w % 4) .. + 31; the first four take the first half of the columns
         if (!offsets) pdl_wait();
-        const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        unsigned char* stage = smem + GM_STAGES * GM_STAGE_BYTES + (warp - 2) * 4096;
+        const bool vec = ((uintptr_t)C & 15) == 0 && ((ldc * (long long)sizeof(TC)) & 15) == 0;
         int local = 0;
         for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++local) {
             int e, mt, m0, m_end, n0;
             place(tile, e, mt, m0, m_end, n0);
-            const int gm = m0 + row;
             bool ok = mbar_wait(&acc_full, local & 1, &abort_flag);
             if (!ok && !abort_flag) { atomicExch(err, GM_ERR_ACC); abort_flag = 1; }
             ok = __all_sync(0xffffffffu, ok);
@@ -295,7 +305,8 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             gm_take<GATED>(tmem_base + ((uint32_t)(quarter * 32) << 16), half, r);
             tc_fence_before();
             mbar_arrive(&acc_empty);
-            if (gm < m_end) gm_give<TC, EPI>(r, C + (size_t)gm * ldc, n0 + (GATED ? 64 : 128) * half, N, glu);
+            if (m0 + quarter * 32 < m_end)
+                gm_give<TC, EPI>(r, stage, lane, C, ldc, m0 + quarter * 32, m_end, n0 + (GATED ? 64 : 128) * half, N, vec, glu);
         }
     }
     __syncwarp();          // the lanes that had no role meet the elected one: the barrier below wants whole warps
@@ -313,7 +324,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 //   * the loads of both CTAs complete on the leader's barrier; a plain bulk copy cannot signal the peer's barrier, so the scales, too, come by
 //     tensor loads, from a map of lines of 1,024 bytes;
 //   * tcgen05.cp.cta_group::2 spreads the scales of each CTA's shared memory over its own tensor memory.
-#define GP_STAGES 6
+#define GP_STAGES 5
 #define GP_STAGE_BYTES (2 * GM_A_BYTES + 3 * MX4_SF_BYTES)          // A, half of B, scales of A, scales of B
 
 __device__ __forceinline__ uint32_t gp_rank() {
@@ -490,7 +501,9 @@ gemm_mx4_pair_kernel(const __grid_constant__ GpMaps maps, TC* C, long long ldc, 
             if (ok) umma_done<2>(on, &acc_full);
         }
     } else if (warp >= 2) {
-        const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        unsigned char* stage = smem + GP_STAGES * GP_STAGE_BYTES + (warp - 2) * 4096;
+        const bool vec = ((uintptr_t)C & 15) == 0 && ((ldc * (long long)sizeof(TC)) & 15) == 0;
         int local = 0;
         for (int tile = pair; tile < total_tiles; tile += n_pairs, ++local) {
             int e, block, m0, m_end, n0;
@@ -506,7 +519,8 @@ gemm_mx4_pair_kernel(const __grid_constant__ GpMaps maps, TC* C, long long ldc, 
             tc_fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gp_leader(&acc_empty)) : "memory");
-            if (m0 + row < m_end) gm_give<TC, EPI>(r, C + (size_t)(m0 + row) * ldc, n0 + (GATED ? 64 : 128) * half, N, glu);
+            if (m0 + quarter * 32 < m_end)
+                gm_give<TC, EPI>(r, stage, lane, C, ldc, m0 + quarter * 32, m_end, n0 + (GATED ? 64 : 128) * half, N, vec, glu);
         }
     }
     __syncwarp();
@@ -544,16 +558,16 @@ static int rllm_gemm_mx4(const void* a_codes, const void* a_scales, const void* 
     if (st) return st;
     auto run = [&](auto one, auto two, auto* out) -> int {
         if (pairs) {
-            constexpr int smem = GP_STAGES * GP_STAGE_BYTES + 1024;
-            const cudaError_t e = cudaFuncSetAttribute(two, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-            if (e != cudaSuccess) return (int)e;
+            constexpr int smem = GP_STAGES * GP_STAGE_BYTES + 8 * 4096 + 1024;
+            const int e = mx4_allow_smem(two, smem);
+            if (e) return e;
             const int n = (int)(most < n_sm / 2 ? most : n_sm / 2);
             return rllm_launch_clusters(two, dim3(2 * n), dim3(GM_THREADS), smem, stream, dim3(2, 1, 1), maps, out, ldc, offsets, E, rows, N, K,
                                         glu, err);
         }
-        constexpr int smem = GM_STAGES * GM_STAGE_BYTES + 1024;
-        const cudaError_t e = cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
+        constexpr int smem = GM_STAGES * GM_STAGE_BYTES + 8 * 4096 + 1024;
+        const int e = mx4_allow_smem(one, smem);
+        if (e) return e;
         return rllm_launch(one, dim3((unsigned)(most < n_sm ? most : n_sm)), dim3(GM_THREADS), smem, stream, maps.a, maps.b,
                            (const uint8_t*)a_scales, (const uint8_t*)b_scales, out, ldc, offsets, E, rows, N, K, ahead, glu, err);
     };

@@ -307,7 +307,7 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            float o = GATED ? glu_apply(glu, sum[0][i], sum[HALVES - 1][i]) : sum[0][i];
+            float o = GATED ? mx4_glu(glu, sum[0][i], sum[HALVES - 1][i]) : sum[0][i];
             if (EPI == GR_EPI_ACCUM) o += old[i];
             if (b0 + i * step < m) dst[(size_t)(i * step) * ldc] = from_f<TC>(o);
         }
@@ -365,12 +365,8 @@ static int gr_launch(const CUtensorMap& tw, const CUtensorMap& tx, const void* s
     constexpr int STAGE_BYTES = 128 * 128 + BN * 128 + 2 * MX4_SF_BYTES, smem = STAGES * STAGE_BYTES + 1024;
     static_assert(BN * 128 * 4 <= STAGES * STAGE_BYTES, "parked sums fit the stages");
     auto kern = gemm_mx4_rows_kernel<BN, STAGES, QW, CTAS, EPI, TC, TX>;
-    static bool attr_set = false;
-    if (!attr_set) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
-        attr_set = true;
-    }
+    const int st = mx4_allow_smem(kern, smem);
+    if (st) return st;
     // chunks of rows: with experts at most one begun chunk for each expert that can have rows beside the full ones
     const long long chunks = so.offsets ? (long long)m / BN + (m < so.E ? m : so.E) : ((long long)m + BN - 1) / BN;
     const int ranks = splits * (EPI == GR_EPI_GATED ? 2 : 1);

@@ -640,9 +640,81 @@ moe_sort_kernel(const int* __restrict__ idx, int n_pairs, int E, int* offsets, i
     }
 }
 
-RLLM_API int rllm_moe_sort(const int* idx, int n_pairs, int E, int* offsets, int* place, cudaStream_t stream) {
+// Up to MOE_SORT_E experts: one block whose 32 warps each take a 32nd of the pairs.  Twice through them, 32 at a time, the lanes that name the
+// same expert found by a ballot for each bit of its number (match.any takes a turn for every expert named): first the counts of every warp,
+// then, from what the experts and the warps before have, the places.  The same order as above (4,000 pairs of 16 experts: 9.9 us there, where a
+// warp walks all pairs for one expert, 5.6 here).
+#define MOE_SORT_E 256
+__device__ __forceinline__ unsigned moe_same(int e, int bits) {
+    unsigned same = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const unsigned set = __ballot_sync(0xffffffffu, (e >> b) & 1);
+        same &= (e >> b) & 1 ? set : ~set;
+    }
+    return same;
+}
+__global__ void __launch_bounds__(1024)
+moe_sort_few_kernel(const int* idx, int n_pairs, int E, int* offsets, int* place) {
+    __shared__ int s_count[32][MOE_SORT_E];
+    __shared__ int s_first[MOE_SORT_E + 1];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int per = ((n_pairs + 31) / 32 + 31) & ~31, first = warp * per, last = min(n_pairs, first + per);
+    const int bits = 32 - __clz(E);
+    for (int e = lane; e < E; e += 32) s_count[warp][e] = 0;
+    __syncwarp();
+    for (int p0 = first; p0 < last; p0 += 32) {
+        const int p = p0 + lane, v = p < last ? idx[p] : E, e = v < 0 || v > E ? E : v;      // (E: none)
+        const unsigned same = moe_same(e, bits);
+        if (e < E && lane == __ffs(same) - 1) s_count[warp][e] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    if (tid < E) {                                           // what the warps before have of this expert, and all of it
+        int run = 0;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) {
+            const int c = s_count[w][tid];
+            s_count[w][tid] = run;
+            run += c;
+        }
+        s_first[tid] = run;
+    }
+    __syncthreads();
+    if (warp == 0) {                                         // exclusive prefix sum over the experts, 32 at a time
+        int run = 0;
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + lane, c = e < E ? s_first[e] : 0;
+            int incl = c;
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, m);
+                if (lane >= m) incl += up;
+            }
+            if (e < E) s_first[e] = run + incl - c;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) s_first[E] = run;
+    }
+    __syncthreads();
+    for (int e = tid; e <= E; e += blockDim.x) offsets[e] = s_first[e];
+    for (int p0 = first; p0 < last; p0 += 32) {
+        const int p = p0 + lane, v = p < last ? idx[p] : E, e = v < 0 || v > E ? E : v;
+        const unsigned same = moe_same(e, bits);
+        const bool mine = e < E;
+        const int at = mine ? s_first[e] + s_count[warp][e] : 0;
+        __syncwarp();
+        if (mine) place[p] = at + __popc(same & ((1u << lane) - 1u));
+        if (mine && lane == __ffs(same) - 1) s_count[warp][e] += __popc(same);
+        __syncwarp();
+    }
+}
+
+RLLM_API int rllm_moe_sort(const int* idx, int* offsets, int* place, int n_pairs, int E, cudaStream_t stream) {
     if (n_pairs <= 0) return 0;
     if (E <= 0 || E > MOE_MAX_EXPERTS) return (int)cudaErrorInvalidValue;
+    if (E <= MOE_SORT_E) return rllm_launch(moe_sort_few_kernel, dim3(1), dim3(1024), 0, stream, idx, n_pairs, E, offsets, place);
     return rllm_launch(moe_sort_kernel, dim3((E + 31) / 32), dim3(1024), 0, stream, idx, n_pairs, E, offsets, place);
 }
 

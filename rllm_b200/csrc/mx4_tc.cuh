@@ -104,7 +104,37 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* r) {
         : "r"(taddr) : "memory");
 }
 
+// glu_apply (common.cuh) with the fast division, 2 ulp where the denominator is below 2^126; beyond it the result is 0 either way.  The
+// clamps leave a NaN what it is.
+__device__ __forceinline__ float mx4_glu(const GluForm& f, float g, float u) {
+    if (f.limit > 0.f) {
+        g = g > f.limit ? f.limit : g;
+        u = u > f.limit ? f.limit : u < -f.limit ? -f.limit : u;
+    }
+    const float z = f.alpha == 0.f ? 1.5957691216057308f * (g + 0.044715f * g * g * g) : f.alpha * g;
+    return __fdividef(g, 1.0f + __expf(-z)) * (u + f.shift);
+}
+
 // ---------------------------------------------------------------- host side
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the runtime once for each of them.
+template <typename F> static int mx4_allow_smem(F* kern, int bytes) {
+    static const void* seen[64];
+    static int seen_device[64], n_seen = 0;
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    for (int i = 0; i < n_seen; ++i)
+        if (seen[i] == (const void*)kern && seen_device[i] == dev) return 0;
+    const cudaError_t s = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (s != cudaSuccess) return (int)s;
+    if (n_seen < 64) {                                   // (two threads at once may each enter it, or lose an entry: asked again then)
+        seen[n_seen] = (const void*)kern;
+        seen_device[n_seen] = dev;
+        ++n_seen;
+    }
+    return 0;
+}
+
 // Tensor map of codes [rows, k / 2] (contiguous): boxes of box_rows x 128 bytes, 128-byte swizzle, zeros outside.
 static inline int mx4_tmap(CUtensorMap* map, const void* base, long long rows, int k, int box_rows) {
     TmapEncodeFn enc = tmap_encoder();

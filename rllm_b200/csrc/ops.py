@@ -1237,14 +1237,17 @@ def moe_pairs_down(act, w_down, idx, weight, out, shared=None, gate=None):
     return out
 
 
+_moe_sort = _Packed("moe", "rllm_moe_sort", 3, 2)
+_moe_combine = _Packed("moe", "rllm_moe_combine", 6, 4)
+
+
 def moe_sort(idx, E):
     """(offsets int32 [E + 1], place int32 [pairs]): the pairs of idx [n, top_k] in expert order (stable)."""
     _need_cuda(idx)
     _need_contig(idx=idx)
     offsets = torch.empty(E + 1, dtype=torch.int32, device=idx.device)
     place = torch.empty(idx.numel(), dtype=torch.int32, device=idx.device)
-    _check(_lib("moe").rllm_moe_sort(_ptr(idx), c_int(idx.numel()), c_int(E), _ptr(offsets), _ptr(place), _stream()),
-           "moe_sort")
+    _check(_moe_sort((idx, offsets, place), (idx.numel(), E)), "moe_sort")
     return offsets, place
 
 
@@ -1297,9 +1300,7 @@ def moe_combine(y, place, weight, out, shared=None, gate=None, top_k=None):
     top_k = weight.shape[1] if weight is not None else int(top_k)
     assert y.dtype == out.dtype == torch.float32 and y.shape == (n * top_k, d)
     assert shared is None or (shared.dtype == torch.float32 and shared.shape == (n, d))
-    _check(_lib("moe").rllm_moe_combine(_ptr(y), _ptr(place), _ptr(weight), _ptr(out), _ptr(shared), _ptr(gate),
-                                        c_longlong(gate.stride(0) if gate is not None else 0), c_int(n), c_int(top_k),
-                                        c_int(d), _stream()), "moe_combine")
+    _check(_moe_combine((y, place, weight, out, shared, gate), (gate.stride(0) if gate is not None else 0, n, top_k, d)), "moe_combine")
     return out
 
 
@@ -1989,7 +1990,7 @@ class Mx4Matrix:
 
     `linear` and `gate_up_swiglu` take one in place of a weight.  settled: the caller knows that no kernel that writes codes or scales is still
     in flight (the weights of a loaded model); products may then read them before the kernels launched before have ended."""
-    __slots__ = ("codes", "scales", "settled", "shape", "device", "is_cuda")
+    __slots__ = ("codes", "scales", "settled", "shape", "device", "is_cuda", "index")
     dtype = torch.uint8
 
     def __init__(self, codes, scales, settled=False):
@@ -2004,7 +2005,10 @@ class Mx4Matrix:
         if not codes.is_contiguous() or not scales.is_contiguous() or (codes.data_ptr() | scales.data_ptr()) % 16:
             raise KernelError("Mx4Matrix: codes and scales must be contiguous and begin at a multiple of 16 bytes")
         self.codes, self.scales, self.settled = codes, scales, settled
-        self.shape, self.device, self.is_cuda = (*lead, n, k), codes.device, codes.is_cuda
+        self.shape, self.device, self.is_cuda, self.index = (*lead, n, k), codes.device, codes.is_cuda, codes.get_device()
+
+    def get_device(self):
+        return self.index
 
     @classmethod
     def from_blocks(cls, codes, scales, settled=False):
@@ -2027,9 +2031,8 @@ class Mx4Matrix:
 
     def dequantize(self, dtype=torch.float32):
         """The values [..., n, k] (exact in float32 and in bfloat16)."""
-        _need_cuda(self)
         _mx4_current(self)
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        out = torch.empty(*self.shape, dtype=dtype, device=self.device)
         code = _code(out)
         *lead, n, k = self.shape
         m = 1
@@ -2054,33 +2057,35 @@ def _mx4_current(*ts):
     """The launchers take the current device's stream: every operand has to be there."""
     here = _current_device()
     for t in ts:
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
+            _need_cuda(t)
             raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{here}")
 
 
 def _mx4_rows(x, who):
     """(rows, entries, stride of the rows) of x [m, k]."""
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise KernelError(f"{who}: rows [m, k] with neighbouring entries side by side, got {tuple(x.shape)} with strides {x.stride()}")
-    m, k = x.shape
-    if k % MX4_BLOCK or k == 0:
-        raise KernelError(f"{who}: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
-    return m, k, x.stride(0)
+    if x.dim() == 2:
+        m, k = x.shape
+        ld, one = x.stride()
+        if one == 1 and k and k % MX4_BLOCK == 0:
+            return m, k, ld
+        if k == 0 or k % MX4_BLOCK:
+            raise KernelError(f"{who}: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
+    raise KernelError(f"{who}: rows [m, k] with neighbouring entries side by side, got {tuple(x.shape)} with strides {x.stride()}")
 
 
 def mx4_quantize(x):
     """x [..., n, k] float32 or bfloat16 (k a multiple of 32; a matrix may have any row stride) as an Mx4Matrix.  A block's scale is 2^(floor(log2 of
     its largest magnitude) - 2), at least 2^-127; entries are rounded to the nearest code, ties to the even one, at most 6 scales; a block
     with an infinity or a NaN becomes NaN.  See mx4.cuh."""
-    _need_cuda(x)
     _mx4_current(x)
     code = _code(x)
     if x.dim() > 2:
         _need_contig(x=x)
     m, k, ld = _mx4_rows(x if x.dim() <= 2 else x.view(-1, x.shape[-1]), "mx4_quantize")
     *lead, n, _ = x.shape
-    codes = torch.empty((*lead, n, k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*lead, *mx4_scale_shape(n, k)), dtype=torch.uint8, device=x.device)
+    codes = torch.empty(*lead, n, k // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*lead, *mx4_scale_shape(n, k), dtype=torch.uint8, device=x.device)
     if m == 0:
         pass
     elif not lead or n % 128 == 0:                     # a stack of whole scale blocks is one matrix as far as the kernel goes
@@ -2092,43 +2097,72 @@ def mx4_quantize(x):
     return Mx4Matrix(codes, scales)
 
 
-MX4_OWN_ROWS = 16              # up to this many rows a product is one launch that quantises them itself,
-MX4_OWN_PAIRS = 256            # and up to this many pairs of tokens and experts
-
-
 def mx4_row_splits(tiles: int, k: int, bn: int, gated: bool, n_sm: int = 148) -> int:
-    """CTAs that share the K of a tile of 128 weight rows in the product of few rows (tiles: with gate and up, experts and chunks of rows
-    counted apart): as many as all run at once, three an SM with up to 32 rows, else two."""
-    most, chunks, s = (3 if bn <= 32 else 2) * n_sm, -(-k // 256), 1
-    while s < (4 if gated else 8) and 2 * s <= chunks and tiles * 2 * s <= most:
+    """CTAs that share the K of a tile of 128 weight rows in the product of few rows; tiles: with gate and up, experts and chunks of rows
+    counted apart.  A CTA keeps a least number of stages of 256 entries, below which the exchange of the sums costs more than it saves, and
+    all CTAs run at once (three an SM with bn 16 and 32, two with 64 and 128).  us with 1 / 2 / 4 / 8:
+        bn 16,  8 rows:   4,096 x 4,096 11.9 / 8.0 / 7.4 / 7.1, 4,096 x 1,024 4.4 / 4.5 / 4.8, 4,096 x 12,288 30.8 / 17.3 / 12.4 / 10.6,
+                          gated 2 x 12,288 x 4,096 17.0 / 12.7 / 21.6
+        bn 32, 16 rows:   4,096 x 4,096 8.4 / 8.0 / 7.7 / 8.8, 1,000 x 2,080 6.0 / 6.7 / 6.6, gated 2 x 12,288 x 4,096 15.1 / 13.9 / 20.5
+        bn 64, 64 rows:   4,096 x 4,096 8.0 / 9.0 / 8.5 / 13.2, 4,096 x 12,288 16.9 / 13.8 / 12.4 / 15.4, gated 2 x 1,536 x 2,048 8.9 / 7.8 / 8.3
+        bn 128, 128 rows: 4,096 x 4,096 9.0 / 11.0 / 11.4, 4,096 x 12,288 23.4 / 19.9 / 17.8, gated 2 x 768 x 2,048 13.0 / 10.8 / 10.4"""
+    chunks = -(-k // 256)
+    if bn == 16:
+        least, most = 2, 3 * n_sm
+    elif gated:
+        least, most = 4, 3 * n_sm if bn == 32 else n_sm
+    elif bn == 32:
+        least, most = 4 if chunks >= 12 else chunks, 3 * n_sm // 2
+    else:
+        least, most = 12, 2 * n_sm
+    s = 1
+    while s < (4 if gated else 8) and chunks >= 2 * s * least and tiles * 2 * s <= most:
         s *= 2
     return s
 
 
 def mx4_few_rows(rows: int, n: int, k: int, gated: bool, own: bool, experts: int = 0, n_sm: int = 148):
-    """(rows of x to a CTA, CTAs that share K) for the product of few rows (gemm_mx4_rows.cu), or None: the one of many rows
-    (gemm_mx4.cu).  own: the rows lie as the kernel that quantises them itself reads them; experts: of sorted rows (0: none)."""
+    """(rows of x to a CTA, CTAs that share K) for the product of few rows (gemm_mx4_rows.cu), or None: the one of many rows (gemm_mx4.cu).
+    own: the rows lie as the kernel that quantises them itself (bn 16) reads them; experts: of sorted rows (0: none).
+    bn 16 is one launch, but every CTA quantises its part of the rows again: up to 8 rows it is as fast as a launch ahead of it (gated
+    8 x 12,288 x 4,096: 12.7 us against 13.9), beyond that with small matrices only (16 x 12,288 x 4,096 gated: 16.6 against 13.9; 16 x 4,096
+    x 1,024: 4.9 against 4.3, where the second launch costs the host more than that).  Sorted rows: while experts have few each (32 pairs of 16
+    experts of 768 x 2,048: 10 us against 18; 400 pairs: 18.8 against 14.7).
+    bn 128 against tiles of 128 x 256, one an SM: as long as its CTAs all run at once, two an SM (512 x 4,096 x 4,096 12.0 us against 13.7,
+    300 x 1,000 x 2,080 8.0 against 10.8, 1,024 x 6,144 x 4,096 21.7 against 22.0); gated, where it takes twice the CTAs, half of that a
+    quarter (256 x 1,536 x 2,048 11.3 against 12.6, 512 rows 14.2 against 13.1)."""
     tiles = -(-n // 128) * (2 if gated else 1)
-    if own and (rows <= MX4_OWN_PAIRS if experts else rows <= MX4_OWN_ROWS):
-        return 16, mx4_row_splits(tiles * min(experts, rows) if experts else tiles, k, 16, gated, n_sm)
-    if experts or rows > MX4_FEW_ROWS:
-        return None
+    if experts:
+        if not own or rows > min(256, 8 * experts):
+            return None
+        return 16, mx4_row_splits(tiles * min(experts, rows), k, 16, gated, n_sm)
+    if own and rows <= 16 and (rows <= 8 or tiles * k <= 1 << 16):
+        return 16, mx4_row_splits(tiles, k, 16, gated, n_sm)
     bn = 32 if rows <= 32 else 64 if rows <= 64 else 128
-    return bn, mx4_row_splits(tiles * -(-rows // bn), k, bn, gated, n_sm)
+    tiles *= -(-rows // bn)
+    if bn == 128 and tiles > (n_sm // 2 if gated else 2 * n_sm):
+        return None
+    return bn, mx4_row_splits(tiles, k, bn, gated, n_sm)
 
 
-MX4_FEW_ROWS = 64
-
-
-def mx4_pairs(rows: int, n: int, gated: bool, experts: int = 0, n_sm: int = 148) -> bool:
-    """Whether the product of many rows takes two SMs to a tile of 256 x 256, or one to a tile of 128 x 256."""
-    return rows > 128 * max(1, experts)
+def mx4_pairs(rows: int, n: int, k: int, gated: bool, experts: int = 0, n_sm: int = 148) -> bool:
+    """Whether the product of many rows takes two SMs to a tile of 256 x 256 (a stage of 256 entries 0.38 us, a tile 1.6 us beside its
+    stages) or one to a tile of 128 x 256 (0.41 us): whichever needs less time for its waves.  us, one / two: 4,096 x 12,288 x 2,048 rows 61.1 /
+    54.6, 4,096 x 4,096: 512 rows 13.7 / 14.2, 2,048 rows 24.1 / 23.6; gated 2 x 12,288 x 4,096: 1,024 rows 54.2 / 49.7, 2,048 rows 93.5 / 87.3;
+    gated 2 x 1,536 x 2,048: 2,048 rows 22.7 / 24.6.  Routed experts seldom fill tiles of 256 rows (4,000 pairs of 16: 18.0 / 21.3)."""
+    if experts:
+        return False
+    cols, stages = -(-n // (128 if gated else 256)), -(-k // 256)
+    one = -(-(-(-rows // 128) * cols) // n_sm) * (0.41 * stages + 1.6)
+    two = -(-(-(-rows // 256) * cols) // (n_sm // 2)) * (0.38 * stages + 1.6) + 1.0
+    return two < one
 
 
 def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, place=None, top_k=0, pairs=None):
     """Checks and launches: x [m, k] (the rows before they are sorted, with `place`), w a stack `lead` of [n, k], out [rows, n].
     few: as mx4_few_rows answers (False for None), by default what it answers."""
-    _need_cuda(x, w, out)
+    if not isinstance(w, Mx4Matrix):
+        raise KernelError(f"{who}: the weight is an Mx4Matrix, not {type(w).__name__}")
     _mx4_current(x, w, out)
     m, k, ldx = _mx4_rows(x, who)
     if out.dim() != 2:
@@ -2154,14 +2188,14 @@ def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, pl
     work = None
     if not few or few[0] != 16:
         work = torch.empty((rows * (k // 2) + 1023 & -1024) + (-(-rows // 128) + experts) * -(-k // 256) * 1024, dtype=torch.uint8,
-                           device=x.device)
+                           device=w.device)
         add_launches(1)
     tensors = (x, offsets, place, w.codes, w.scales, out, work, err)
     if few:
         st = _mx4_few(tensors, (ldx if m > 1 else 0, ldc, x_code, out_code, rows, n, k, experts, top_k, epilogue, *few, ahead), glu)
     else:
         if pairs is None:
-            pairs = mx4_pairs(rows, n, epilogue == EPI_SWIGLU, experts, sm_count(x.device))
+            pairs = mx4_pairs(rows, n, k, epilogue == EPI_SWIGLU, experts, sm_count(x.device))
         st = _mx4_many(tensors, (ldx, ldc, x_code, out_code, rows, n, k, experts or 1, top_k, epilogue, int(pairs), ahead), glu)
     if st >= 30000:
         raise KernelError(f"{who}: tensor map encoding failed (CUresult {st - 30000})")
@@ -2178,7 +2212,7 @@ def mx4_linear(x, w, out=None, out_dtype=None, accumulate=False):
     if out is None:
         if accumulate:
             raise KernelError("mx4_linear: accumulate needs an output to add to")
-        out = torch.empty((x.shape[0], w.shape[-2]), dtype=out_dtype or x.dtype, device=x.device)
+        out = torch.empty(x.shape[0], w.shape[-2], dtype=out_dtype or x.dtype, device=w.device)
     return _mx4_product(x, w, out, (), EPI_ACCUM if accumulate else EPI_STORE, _SWIGLU, "mx4_linear")
 
 
@@ -2193,7 +2227,6 @@ def _mx4_experts(experts, rows, offsets, place, who):
         raise KernelError(f"{who}: {experts} experts (1 to {MX4_MAX_EXPERTS})")
     for name, t, size in (("offsets", offsets, experts + 1), ("place", place, rows)):
         if t is not None:
-            _need_cuda(t)
             _mx4_current(t)
             if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != size:
                 raise KernelError(f"{who}: {name} is int32 [{size}]")
