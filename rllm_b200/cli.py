@@ -2,7 +2,7 @@
 
   rllm run MODEL PROMPT [-n/--max-tokens 256] [-t/--temperature 0] [--top-k 0] [--top-p 1.0]
                         [--seed 0] [--ctx 4096] [--block-size 32] [--prefill-chunk 512]
-                        [--kv-type bf16|f32] [--show-ids]
+                        [--kv-type bf16|f32] [--weights mxfp4] [--show-ids]
   rllm bench MODEL [-p/--n-prompt 512] [-n/--n-gen 128] [-r/--reps 3] [--depth 0] [-b/--batch 1]
   rllm compare MODEL PROMPT [-n/--steps 32]      engine float32 against engine bfloat16, same tokens
   rllm compare-ref MODEL DUMP [--prefill-chunk 512]
@@ -15,7 +15,8 @@
 
 The engine has no tokenizer: PROMPT is token ids separated by commas or spaces, or @FILE holding
 them.  MODEL is a folder with config.json and model.safetensors.  ``--kv-type`` chooses the
-precision of the whole engine (bf16 serving path, f32 true 32-bit path).
+precision of the whole engine (bf16 serving path, f32 true 32-bit path).  ``--weights mxfp4`` (run, bench,
+compare, compare-ref, perplexity; with bf16) keeps the matrices in microscaled 4-bit numbers.
 """
 from __future__ import annotations
 
@@ -44,7 +45,7 @@ def cmd_run(a) -> int:
         return 2
     t0 = time.time()
     llm = LLM(a.model, dtype=_dtype(a.kv_type), device=a.device, ctx=a.ctx, block_size=a.block_size,
-              prefill_chunk=a.prefill_chunk, parallel=1, host_sampling=a.host_sampling)
+              prefill_chunk=a.prefill_chunk, parallel=1, host_sampling=a.host_sampling, weights=a.weights)
     print(f"[rllm] loaded in {time.time() - t0:.2f} s", file=sys.stderr)
     t0 = time.time()
     out = llm.generate([prompt], max_tokens=a.max_tokens, temperature=a.temperature, top_k=a.top_k,
@@ -62,7 +63,7 @@ def cmd_bench(a) -> int:
     import torch
     from .engine import Engine, StepItem
     from .models.model import load_model
-    _, model = load_model(a.model, _dtype(a.kv_type), a.device)
+    _, model = load_model(a.model, _dtype(a.kv_type), a.device, a.weights)
     V = model.spec.vocab_size
     per_req = max(a.depth, 0) + a.n_prompt + a.n_gen
     eng = Engine(model, block_size=a.block_size, max_tokens=(per_req + 64) * a.batch, max_requests=a.batch)
@@ -103,7 +104,7 @@ def cmd_compare(a) -> int:
     prompt = _ids(a.prompt)
     engines = []
     for dt in ("float32", "bfloat16"):
-        _, m = load_model(a.model, dt, a.device)
+        _, m = load_model(a.model, dt, a.device, a.weights if dt == "bfloat16" else None)
         engines.append(Engine(m, block_size=a.block_size, max_tokens=len(prompt) + a.steps + 64, max_requests=1))
     feed, worst, mism = prompt, 0.0, 0
     for i in range(a.steps + 1):
@@ -155,7 +156,7 @@ def cmd_compare_ref(a) -> int:
     from .engine import Engine, StepItem
     from .models.model import load_model
     n_vocab, n_prompt, tokens, ref = read_ref_dump(a.reference)
-    _, model = load_model(a.model, _dtype(a.kv_type), a.device)
+    _, model = load_model(a.model, _dtype(a.kv_type), a.device, a.weights)
     if model.spec.vocab_size != n_vocab:
         print(f"vocab mismatch: model {model.spec.vocab_size} vs reference {n_vocab}", file=sys.stderr)
         return 2
@@ -204,7 +205,7 @@ def cmd_perplexity(a) -> int:
         print(f"need at least {2 * n_ctx} tokens for --ctx {n_ctx}", file=sys.stderr)
         return 2
     n_chunk = min(len(tokens) // n_ctx, a.chunks or 1 << 60)
-    _, model = load_model(a.model, _dtype(a.kv_type), a.device)
+    _, model = load_model(a.model, _dtype(a.kv_type), a.device, a.weights)
     eng = Engine(model, block_size=a.block_size, max_tokens=n_ctx + 64, max_requests=1)
     first = n_ctx // 2
     rows = list(range(first, n_ctx - 1))
@@ -264,6 +265,8 @@ def main(argv=None) -> int:
         p.add_argument("-d", "--device", default="cuda:0")
         p.add_argument("--block-size", type=int, default=32)
         p.add_argument("--kv-type", default="bf16", choices=["bf16", "f32", "bfloat16", "float32"])
+        p.add_argument("--weights", default=None, choices=["mxfp4"],
+                       help="quantise the matrices to 4 bits when they are loaded (compare: those of the bfloat16 engine)")
 
     p = sub.add_parser("run"); common(p)
     p.add_argument("prompt")

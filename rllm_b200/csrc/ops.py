@@ -2053,13 +2053,17 @@ _mx4_many = _Packed("mx4", "rllm_mx4_product", 8, 12, 3)
 _mx4_few = _Packed("mx4_rows", "rllm_mx4_rows_product", 8, 13, 3)
 
 
-def _mx4_current(*ts):
+def _mx4_current(first, *others):
     """The launchers take the current device's stream: every operand has to be there."""
-    here = _current_device()
-    for t in ts:
-        if t is not None and t.get_device() != here:
-            _need_cuda(t)
-            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{here}")
+    at = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != at:
+            _need_cuda(first, *others)
+            raise KernelError(f"operands on {first.device} and on {t.device}")
+    if at < 0:
+        _need_cuda(first)
+    if at != _current_device():
+        raise KernelError(f"a tensor is on {first.device}, the current device is cuda:{_current_device()}")
 
 
 def _mx4_rows(x, who):

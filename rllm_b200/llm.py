@@ -7,7 +7,10 @@ names and meanings where it has them (crates/rllm-cli/src/main.rs:39-110, 195-23
 ctx * parallel), ``max_tokens`` (256), ``temperature`` (0 = greedy), ``top_k`` (0 = off),
 ``top_p`` (1.0 = off), ``seed`` (0), ``frequency_penalty`` / ``presence_penalty`` / ``logit_bias``
 (the request parameters of the reference's server), ``host_sampling`` (sample on the host from copied logits
-instead of on the device).
+instead of on the device), ``weights`` ("mxfp4": the matrices of attention, feed-forwards and gated experts in
+microscaled 4-bit numbers, quantised when the model is loaded, and the rows that meet them likewise: a quarter of
+the bytes a decode step reads and the 4-bit rate of the tensor cores for prompts, with the precision of 4 bits;
+None: as stored).
 """
 from __future__ import annotations
 
@@ -50,11 +53,13 @@ class _SampledIds:
 class LLM:
     def __init__(self, model, dtype="bfloat16", device="cuda:0", ctx: int = 4096, block_size: int = 32,
                  prefill_chunk: int = 512, parallel: int = 4, kv_tokens: Optional[int] = None,
-                 host_sampling: bool = False):
+                 host_sampling: bool = False, weights: Optional[str] = None):
         """`model`: a folder with config.json and model.safetensors, or a loaded DecoderModel."""
         if isinstance(model, (str, bytes)) or hasattr(model, "__fspath__"):
-            self.config, self.model = load_model(model, dtype, device)
+            self.config, self.model = load_model(model, dtype, device, weights)
         else:
+            if weights is not None and weights != model.runtime.weights:
+                raise ValueError("weights: the model is loaded already, with weights " + repr(model.runtime.weights))
             self.config, self.model = None, model
         limit = int(getattr(self.model.spec, "max_position", 0) or 0)
         if limit and ctx > limit:
@@ -212,11 +217,12 @@ def generate(model, prompts, max_tokens: int = 256, temperature: float = 0.0, to
              top_p: float = 1.0, seed: int = 0, dtype="bfloat16", device="cuda:0", ctx: int = 4096,
              block_size: int = 32, prefill_chunk: int = 512, parallel: int = 4,
              kv_tokens: Optional[int] = None, stop_ids=(), host_sampling: bool = False,
-             frequency_penalty: float = 0.0, presence_penalty: float = 0.0, logit_bias=()):
+             frequency_penalty: float = 0.0, presence_penalty: float = 0.0, logit_bias=(),
+             weights: Optional[str] = None):
     """One call: load `model` (a folder), generate for `prompts` (lists of token ids)."""
     llm = LLM(model, dtype=dtype, device=device, ctx=ctx, block_size=block_size,
               prefill_chunk=prefill_chunk, parallel=parallel, kv_tokens=kv_tokens,
-              host_sampling=host_sampling)
+              host_sampling=host_sampling, weights=weights)
     return llm.generate(prompts, max_tokens=max_tokens, temperature=temperature, top_k=top_k,
                         top_p=top_p, seed=seed, stop_ids=stop_ids, frequency_penalty=frequency_penalty,
                         presence_penalty=presence_penalty, logit_bias=logit_bias)

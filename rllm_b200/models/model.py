@@ -20,7 +20,12 @@ TRACE_LAYERS = os.environ.get("RLLM_B200_NO_LAYER_TRACE", "0") in ("", "0")
 
 def _tensors_of(obj) -> dict:
     """attribute name -> device tensor of an object (a part's weights, a cache view's planes)."""
-    return {k: v for k, v in vars(obj).items() if isinstance(v, torch.Tensor) and v.is_cuda}
+    from ..csrc import ops
+    out = {k: v for k, v in vars(obj).items() if isinstance(v, torch.Tensor) and v.is_cuda}
+    for k, v in vars(obj).items():
+        if isinstance(v, ops.Mx4Matrix):
+            out[k + ".codes"], out[k + ".scales"] = v.codes, v.scales
+    return out
 
 
 class _LayerTrace:
@@ -134,6 +139,14 @@ class DecoderModel:
             p.load(tensors)
         shared[getattr(self.embedding, "name", self.embedding.prefix + "weight")] = self.embedding.weight
         self.lm_head.load(tensors, shared=shared)
+        if self.runtime.weights is not None:
+            from ..csrc import ops
+            four = [v for p in self._weighted_parts() for v in vars(p).values() if isinstance(v, ops.Mx4Matrix)]
+            if not four:
+                raise ValueError(f"weights '{self.runtime.weights}': no part of this model keeps its matrices in 4 bits")
+            torch.cuda.synchronize(self.runtime.device)       # the kernels that wrote them have ended: products may read them ahead
+            for v in four:
+                v.settled = True
         self.loaded = True
 
     def load_dir(self, model_dir) -> None:
@@ -222,20 +235,21 @@ def parse_dtype(dtype) -> torch.dtype:
     raise ValueError(f"dtype must be bfloat16 or float32, got {dtype!r}")
 
 
-def load_model(model_dir, dtype="bfloat16", device="cuda:0"):
+def load_model(model_dir, dtype="bfloat16", device="cuda:0", weights=None):
     """config.json chooses the model class (through the architecture registry); weights come from
-    model.safetensors.  Returns (config, DecoderModel)."""
+    model.safetensors (`weights` "mxfp4": the matrices of attention, feed-forwards and gated experts are
+    quantised to 4 bits on the way, see Runtime).  Returns (config, DecoderModel)."""
     config = load_config(model_dir)
-    model = DecoderModel(config.model_spec(), Runtime(torch.device(device), parse_dtype(dtype)))
+    model = DecoderModel(config.model_spec(), Runtime(torch.device(device), parse_dtype(dtype), weights))
     model.load_dir(Path(model_dir))
     return config, model
 
 
 def random_model(config: ModelConfig, seed=0, dtype="bfloat16", device="cuda:0", std=0.02, norm_std=0.1,
-                 generate_on_device=False):
+                 generate_on_device=False, weights=None):
     """A model with random weights without going through a file (large benchmarks)."""
     from ..weights.random_init import random_tensors
-    rt = Runtime(torch.device(device), parse_dtype(dtype))
+    rt = Runtime(torch.device(device), parse_dtype(dtype), weights)
     model = DecoderModel(config.model_spec(), rt)
     tensors = random_tensors(model.expected_tensors(), seed, rt.dtype, std, norm_std,
                              device=device if generate_on_device else "cpu")

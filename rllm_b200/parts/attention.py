@@ -103,10 +103,10 @@ class Attention(Mixer):
             out[:, :size] = t.view(heads, size, t.shape[1])
             return out.view(heads * to, t.shape[1])
         sizes = {"q": (self.H, self.hd, self.hd_s), "k": (self.K, self.hd, self.hd_s), "v": (self.K, self.hdv, self.hdv_s)}
-        self.w_qkv = self._to_device(torch.cat([stored(tensors[n[s]].to(dt), *sizes[s])
-                                                for s in ("qkv" if self.own_kv else "q")], 0))
-        self.w_o = self._to_device(stored(tensors[n["o"]].t().contiguous(), self.H, self.hdv, self.hdv_s).t()
-                                   if self.hdv_s != self.hdv else tensors[n["o"]])
+        self.w_qkv = self._matrix(torch.cat([stored(tensors[n[s]].to(dt), *sizes[s])
+                                             for s in ("qkv" if self.own_kv else "q")], 0))
+        self.w_o = self._matrix(stored(tensors[n["o"]].t().contiguous(), self.H, self.hdv, self.hdv_s).t()
+                                if self.hdv_s != self.hdv else tensors[n["o"]])
         if self.qk_norm:
             self.q_norm_w = self._to_device(tensors[n["q.norm"]], torch.float32)
             if self.own_kv:

@@ -49,9 +49,20 @@ def build_part(category: str, spec, runtime: "Runtime", **extra):
 class Runtime:
     """Where and in which precision a model runs.  `dtype` is the storage type of weights,
     activations between kernels and the cache (bfloat16 or float32); the residual stream,
-    norms' statistics, softmax, rotation angles and logits are float32 in both."""
+    norms' statistics, softmax, rotation angles and logits are float32 in both.
+
+    `weights` "mxfp4" (with bfloat16): the matrices of the parts that say so (`Part._matrix`: attention, feed-forwards and gated
+    routed experts) are quantised to microscaled 4-bit numbers when they are loaded, and so are the rows that meet them, by the
+    products themselves (csrc/ops.Mx4Matrix); all else keeps `dtype`."""
     device: torch.device
     dtype: torch.dtype
+    weights: Optional[str] = None
+
+    def __post_init__(self):
+        if self.weights not in (None, "mxfp4"):
+            raise PartError(f"weights must be None or 'mxfp4', got {self.weights!r}")
+        if self.weights is not None and self.dtype != torch.bfloat16:
+            raise PartError(f"weights '{self.weights}' go with bfloat16 activations, not {self.dtype}")
 
     @property
     def is_f32(self) -> bool:
@@ -117,6 +128,19 @@ class Part:
 
     def _to_device(self, t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return t.to(device=self.runtime.device, dtype=dtype or self.runtime.dtype).contiguous()
+
+    def _matrix(self, t: torch.Tensor, halves: int = 1):
+        """A product's weight [..., n, k] on the device: as `_to_device`, or as 4-bit numbers where the runtime asks for them; the gate
+        and up rows of a gated product (halves 2: [..., 2 n, k]) are then a stack of their own, [..., 2, n, k]."""
+        if self.runtime.weights is None:
+            return self._to_device(t)
+        from ..csrc import ops
+        if t.shape[-1] % ops.MX4_BLOCK:
+            raise PartError(f"{self.prefix or type(self).__name__}: 4-bit weights come in blocks of {ops.MX4_BLOCK} entries, "
+                            f"a matrix here has rows of {t.shape[-1]}")
+        w = self._to_device(t)
+        with torch.cuda.device(w.device):
+            return ops.mx4_quantize(w if halves == 1 else w.view(*w.shape[:-2], halves, w.shape[-2] // halves, w.shape[-1]))
 
 
 class Mixer(Part):

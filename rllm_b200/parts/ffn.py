@@ -37,8 +37,8 @@ class SwiGLU(FeedForward):
     def load(self, tensors):
         g = tensors[self.prefix + "gate_proj.weight"]
         u = tensors[self.prefix + "up_proj.weight"]
-        self.w_gate_up = self._to_device(torch.cat([g.to(self.runtime.dtype), u.to(self.runtime.dtype)], 0))
-        self.w_down = self._to_device(tensors[self.prefix + "down_proj.weight"])
+        self.w_gate_up = self._matrix(torch.cat([g.to(self.runtime.dtype), u.to(self.runtime.dtype)], 0), halves=2)
+        self.w_down = self._matrix(tensors[self.prefix + "down_proj.weight"])
 
     def first_product(self):
         return self.w_gate_up, True
@@ -80,8 +80,8 @@ class DenseAct(FeedForward):
         return {self.prefix + "up": ((F, d), "matrix"), self.prefix + "down": ((d, F), "matrix")}
 
     def load(self, tensors):
-        self.w_up = self._to_device(tensors[self.prefix + "up"])
-        self.w_down = self._to_device(tensors[self.prefix + "down"])
+        self.w_up = self._matrix(tensors[self.prefix + "up"])
+        self.w_down = self._matrix(tensors[self.prefix + "down"])
 
     def forward(self, h, ctx=None, residual=None):
         up = ops.linear(h, self.w_up, out_dtype=torch.float32)
@@ -126,8 +126,8 @@ class ClampedGLU(FeedForward):
 
     def load(self, tensors):
         p, dt = self.prefix, self.runtime.dtype
-        self.w_gate_up = self._to_device(torch.cat([tensors[p + "gate"].to(dt), tensors[p + "up"].to(dt)], 0))
-        self.w_down = self._to_device(tensors[p + "down"])
+        self.w_gate_up = self._matrix(torch.cat([tensors[p + "gate"].to(dt), tensors[p + "up"].to(dt)], 0), halves=2)
+        self.w_down = self._matrix(tensors[p + "down"])
 
     def forward(self, h, ctx=None, residual=None):
         act = torch.empty((h.shape[0], self.intermediate_size), dtype=self.runtime.dtype, device=h.device)

@@ -32,6 +32,7 @@ Steps of few rows run every (token, chosen expert) pair against its expert's mat
 host involvement (so such steps can be captured into graphs).  Steps of many rows sort the pairs by
 expert on the device; experts without a gate then run as two grouped products (one launch each, no host involvement), gated
 ones, float32 and odd sizes by reading the experts' counts back and running each expert's rows through the package's products.
+Gated experts with 4-bit weights (Runtime.weights) run as two grouped products whatever the number of rows.
 """
 from __future__ import annotations
 
@@ -111,12 +112,14 @@ class RoutedExperts(FeedForward):
             self.correction = self._to_device(tensors[p + "correction"], torch.float32)
         if self.has_bias:
             self.router_bias = self._to_device(tensors[p + "router.b"], torch.float32)
-        self.w_gu = self._to_device(torch.stack(
-            [torch.cat([tensors[f"{p}e{e}.{s}"].to(dt) for s in self.parts_up], 0) for e in range(self.E)], 0))
-        self.w_down = self._to_device(torch.stack([tensors[f"{p}e{e}.down"].to(dt) for e in range(self.E)], 0))
+        # (experts without a gate keep the runtime's type where the runtime asks for 4-bit weights)
+        matrix = (lambda t, halves=1: self._to_device(t)) if self.activation is not None else self._matrix
+        self.w_gu = matrix(torch.stack(
+            [torch.cat([tensors[f"{p}e{e}.{s}"].to(dt) for s in self.parts_up], 0) for e in range(self.E)], 0), halves=2)
+        self.w_down = matrix(torch.stack([tensors[f"{p}e{e}.down"].to(dt) for e in range(self.E)], 0))
         if self.shared_size:
-            self.w_shared_gu = self._to_device(torch.cat([tensors[f"{p}shared.{s}"].to(dt) for s in self.parts_up], 0))
-            self.w_shared_down = self._to_device(tensors[p + "shared.down"])
+            self.w_shared_gu = matrix(torch.cat([tensors[f"{p}shared.{s}"].to(dt) for s in self.parts_up], 0), halves=2)
+            self.w_shared_down = matrix(tensors[p + "shared.down"])
 
     def route(self, h):
         """(idx int32 [n, top_k], weight float32 [n, top_k], logits float32 [n, E (+ 1), padded to a multiple of 8])."""
@@ -144,6 +147,13 @@ class RoutedExperts(FeedForward):
             shared = ops.linear(act, self.w_shared_down, out_dtype=torch.float32)
             gate = logits[:, self.E:self.E + 1] if self.shared_gate else None
         out = torch.empty((n, d), dtype=torch.float32, device=dev)
+        if isinstance(self.w_gu, ops.Mx4Matrix):               # any number of rows: sorted, through both products, and back
+            offsets, place = ops.moe_sort(idx, self.E)
+            act = torch.empty((n * self.top_k, self.F), dtype=dt, device=dev)
+            ops.mx4_experts_up(h, self.w_gu, offsets, place, act, glu=self.expert_form)
+            y = torch.empty((n * self.top_k, d), dtype=torch.float32, device=dev)
+            ops.mx4_experts_down(act, self.w_down, offsets, y)
+            return ops.moe_combine(y, place, weight, out, shared, gate, self.top_k)
         if few:
             act = torch.empty((n * self.top_k, self.F), dtype=dt, device=dev)
             if self.activation is not None:
