@@ -8,6 +8,7 @@ cannot be built and loaded, raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
@@ -255,7 +256,7 @@ class _Packed:
 
     def __call__(self, tensors, integers, floats=()):
         if _trace is None and self._fn is not None:
-            return self._fn(self._pack(*[0 if t is None else t.data_ptr() for t in tensors], *integers, *floats,
+            return self._fn(self._pack(*[t.data_ptr() if t is not None else 0 for t in tensors], *integers, *floats,
                                        _raw_stream(_current_device())))
         lib = _lib(self.library)
         if _trace is None and not profiler.enabled():
@@ -1994,18 +1995,22 @@ class Mx4Matrix:
     dtype = torch.uint8
 
     def __init__(self, codes, scales, settled=False):
-        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.dim() < 2 or scales.dim() != codes.dim() + 3:
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.dim() < 2:
             raise KernelError("Mx4Matrix: codes are uint8 [..., n, k / 2], scales uint8 [..., n / 128, k / 128, 32, 4, 4]")
         *lead, n, half = codes.shape
         k = 2 * half
         if k % MX4_BLOCK or k == 0:
             raise KernelError(f"Mx4Matrix: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
-        if tuple(scales.shape) != (*lead, -(-n // 128), 2 * -(-k // 256), 32, 4, 4) or scales.device != codes.device:
+        if scales.shape != (*lead, n + 127 >> 7, 2 * (k + 255 >> 8), 32, 4, 4) or scales.get_device() != codes.get_device():
             raise KernelError(f"Mx4Matrix: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)}")
-        if not codes.is_contiguous() or not scales.is_contiguous() or (codes.data_ptr() | scales.data_ptr()) % 16:
+        if not (codes.is_contiguous() and scales.is_contiguous()) or (codes.data_ptr() | scales.data_ptr()) & 15:
             raise KernelError("Mx4Matrix: codes and scales must be contiguous and begin at a multiple of 16 bytes")
-        self.codes, self.scales, self.settled = codes, scales, settled
-        self.shape, self.device, self.is_cuda, self.index = (*lead, n, k), codes.device, codes.is_cuda, codes.get_device()
+        self._set(codes, scales, (*lead, n, k), settled)
+
+    def _set(self, codes, scales, shape, settled=False):
+        self.codes, self.scales, self.shape, self.settled = codes, scales, shape, settled
+        self.device, self.is_cuda, self.index = codes.device, codes.is_cuda, codes.get_device()
+        return self
 
     def get_device(self):
         return self.index
@@ -2098,7 +2103,7 @@ def mx4_quantize(x):
         parts = codes.view(-1, n, k // 2), scales.view(-1, *scales.shape[-5:])
         for rows, c, s in zip(x.view(-1, n, k), *parts):
             _check(_mx4_quantize((rows, c, s, None, None), (k, code, n, k, 1, 0, 0)), "mx4_quantize")
-    return Mx4Matrix(codes, scales)
+    return Mx4Matrix.__new__(Mx4Matrix)._set(codes, scales, (*lead, n, k))
 
 
 def mx4_row_splits(tiles: int, k: int, bn: int, gated: bool, n_sm: int = 148) -> int:
@@ -2125,6 +2130,7 @@ def mx4_row_splits(tiles: int, k: int, bn: int, gated: bool, n_sm: int = 148) ->
     return s
 
 
+@functools.lru_cache(maxsize=4096)
 def mx4_few_rows(rows: int, n: int, k: int, gated: bool, own: bool, experts: int = 0, n_sm: int = 148):
     """(rows of x to a CTA, CTAs that share K) for the product of few rows (gemm_mx4_rows.cu), or None: the one of many rows (gemm_mx4.cu).
     own: the rows lie as the kernel that quantises them itself (bn 16) reads them; experts: of sorted rows (0: none).
@@ -2174,8 +2180,10 @@ def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, pl
     rows, n = out.shape
     if w.shape != (*lead, n, k):
         raise KernelError(f"{who}: a weight {w.shape} where {(*lead, n, k)} is needed")
-    ldc = out.stride(0) if rows > 1 else n
-    if (n > 1 and out.stride(1) != 1) or ldc < n:
+    ldc, one = out.stride()
+    if rows <= 1:
+        ldc = n
+    if (n > 1 and one != 1) or ldc < n:
         raise KernelError(f"{who}: an output with strides {out.stride()} for {n} columns")
     if rows != (m if place is None else m * top_k):
         raise KernelError(f"{who}: an output of {rows} rows for {m} rows" + (f" and {top_k} experts each" if place is not None else ""))
@@ -2184,26 +2192,31 @@ def _mx4_product(x, w, out, lead, epilogue, glu, who, few=None, offsets=None, pl
         raise KernelError("accumulating product needs a float32 output")
     if rows == 0 or n == 0:
         return out
-    err, ahead = error_word(x.device), 1 if w.settled else 0
+    err = _error_words.get(w.index)
+    if err is None:
+        err = error_word(x.device)
     experts = lead[0] if offsets is not None else 0
+    n_sm = _n_sm.get(w.index) or sm_count(x.device)
     if few is None:
-        own = x.data_ptr() % 16 == 0 and (m == 1 or ldx * x.element_size() % 16 == 0)
-        few = mx4_few_rows(rows, n, k, epilogue == EPI_SWIGLU, own, experts, sm_count(x.device))
+        own = x.data_ptr() & 15 == 0 and (m == 1 or ldx * x.element_size() & 15 == 0)
+        few = mx4_few_rows(rows, n, k, epilogue == EPI_SWIGLU, own, experts, n_sm)
     work = None
     if not few or few[0] != 16:
-        work = torch.empty((rows * (k // 2) + 1023 & -1024) + (-(-rows // 128) + experts) * -(-k // 256) * 1024, dtype=torch.uint8,
+        work = torch.empty((rows * (k // 2) + 1023 & -1024) + ((rows + 127 >> 7) + experts) * (k + 255 >> 8) * 1024, dtype=torch.uint8,
                            device=w.device)
         add_launches(1)
     tensors = (x, offsets, place, w.codes, w.scales, out, work, err)
     if few:
-        st = _mx4_few(tensors, (ldx if m > 1 else 0, ldc, x_code, out_code, rows, n, k, experts, top_k, epilogue, *few, ahead), glu)
+        st = _mx4_few(tensors, (ldx if m > 1 else 0, ldc, x_code, out_code, rows, n, k, experts, top_k, epilogue, *few, w.settled), glu)
     else:
         if pairs is None:
-            pairs = mx4_pairs(rows, n, k, epilogue == EPI_SWIGLU, experts, sm_count(x.device))
-        st = _mx4_many(tensors, (ldx, ldc, x_code, out_code, rows, n, k, experts or 1, top_k, epilogue, int(pairs), ahead), glu)
-    if st >= 30000:
-        raise KernelError(f"{who}: tensor map encoding failed (CUresult {st - 30000})")
-    _check(st, who)
+            pairs = mx4_pairs(rows, n, k, epilogue == EPI_SWIGLU, experts, n_sm)
+        st = _mx4_many(tensors, (ldx, ldc, x_code, out_code, rows, n, k, experts or 1, top_k, epilogue, pairs, w.settled), glu)
+    if st:
+        if st >= 30000:
+            raise KernelError(f"{who}: tensor map encoding failed (CUresult {st - 30000})")
+        _check(st, who)
+    add_launches(1)
     return out
 
 
