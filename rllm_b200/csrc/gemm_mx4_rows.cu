@@ -30,15 +30,19 @@ template <> struct RowPart<bf16> {
     uint4 u;
     __device__ __forceinline__ void load(const bf16* p) { u = *reinterpret_cast<const uint4*>(p); }
     __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void get(float (&v)[8]) const { mx4_unpack(u, v); }
+    __device__ __forceinline__ uint32_t codes(int lane, uint32_t& word) const {
+        float v[8];
+        mx4_unpack(u, v);
+        return mx4_quantize8(v, mx4_top8(u), lane, word);
+    }
 };
 template <> struct RowPart<float> {
     float4 a, b;
     __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
     __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    __device__ __forceinline__ uint32_t codes(int lane, uint32_t& word) const {
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        return mx4_quantize8(v, mx4_top8(v), lane, word);
     }
 };
 
@@ -235,9 +239,7 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
 #pragma unroll
                         for (int j = 0; j < RPW; ++j) {
                             if (j && first + QW * j >= m) break;
-                            float f[8];
-                            part[d][j].get(f);
-                            code[j] = mx4_quantize8(f, lane, word[j]);
+                            code[j] = part[d][j].codes(lane, word[j]);
                         }
                         if (!mbar_wait(&empty_bar[s], ((i / STAGES) & 1) ^ 1, &abort_flag)) {
                             if (!abort_flag) { atomicExch(err, GR_ERR_EMPTY); abort_flag = 1; }

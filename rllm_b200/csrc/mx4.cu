@@ -22,7 +22,11 @@ template <> struct MqPart<bf16> {
         u = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
     }
     __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void get(float (&v)[8]) const { mx4_unpack(u, v); }
+    __device__ __forceinline__ uint32_t codes(int lane, uint32_t& word) const {
+        float v[8];
+        mx4_unpack(u, v);
+        return mx4_quantize8(v, mx4_top8(u), lane, word);
+    }
 };
 template <> struct MqPart<float> {
     float v8[8];
@@ -31,10 +35,7 @@ template <> struct MqPart<float> {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v8[i] = 0.f;
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v8[i];
-    }
+    __device__ __forceinline__ uint32_t codes(int lane, uint32_t& word) const { return mx4_quantize8(v8, mx4_top8(v8), lane, word); }
 };
 
 template <typename T, bool VEC, bool SORTED>
@@ -60,10 +61,11 @@ mx4_quantize_kernel(const T* x, long long ld, int rows, int k, uint8_t* codes, u
     }
     MqPart<T> part[MQ_RUNS];
     const bool here = item < (unsigned)rows;                     // (rows behind the last one get scales of zero)
+    const int col0 = c0 * MX4_CHUNK + lane * 8, left = here ? k - col0 : 0;      // (k is a multiple of 32: a lane's eight are all in or all out)
+    const T* from = x + src * ld + col0;
 #pragma unroll
     for (int i = 0; i < MQ_RUNS; ++i) {
-        const int col = (c0 + i) * MX4_CHUNK + lane * 8;         // (k is a multiple of 32: a lane's eight are all in or all out)
-        if (here && col < k) part[i].template load<VEC>(x + src * ld + col);
+        if (i * MX4_CHUNK < left) part[i].template load<VEC>(from + i * MX4_CHUNK);
         else part[i].zero();
     }
     if (SORTED) {
@@ -86,17 +88,15 @@ mx4_quantize_kernel(const T* x, long long ld, int rows, int k, uint8_t* codes, u
         // (offsets that do not rise from 0 to the number of rows: nothing outside the scales is written)
         if (scale_row < 0 || scale_row >= ((long long)((rows + 127) >> 7) + E) * 128) return;
     }
+    uint8_t* code_to = codes + row * (long long)(k >> 1) + (col0 >> 1);
+    uint8_t* scale_to = scales + mx4_scale_at(scale_row, (long long)c0 * 8 + (lane >> 4) * 4, 2ll * chunks);
 #pragma unroll
     for (int i = 0; i < MQ_RUNS; ++i) {
-        const int c = c0 + i, col = c * MX4_CHUNK + lane * 8;
-        if (c >= chunks) break;
-        float v[8];
-        part[i].get(v);
+        if (c0 + i >= chunks) break;
         uint32_t word;
-        const uint32_t code = mx4_quantize8(v, lane, word);
-        if (here && col < k) *reinterpret_cast<uint32_t*>(codes + row * (long long)(k >> 1) + (col >> 1)) = code;
-        if ((lane & 15) == 0)
-            *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(scale_row, (long long)c * 8 + (lane >> 4) * 4, 2ll * chunks)) = word;
+        const uint32_t code = part[i].codes(lane, word);
+        if (i * MX4_CHUNK < left) *reinterpret_cast<uint32_t*>(code_to + i * (MX4_CHUNK / 2)) = code;
+        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scale_to + i * 2 * MX4_ATOM) = word;
     }
 }
 

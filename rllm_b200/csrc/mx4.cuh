@@ -45,27 +45,39 @@ __device__ __forceinline__ uint32_t mx4_encode8(const float (&v)[8]) {
     return r;
 }
 
+// The bits of the largest magnitude among eight entries (a NaN's are above an infinity's, and those above every number's).
 __device__ __forceinline__ uint32_t mx4_top8(const float (&v)[8]) {
     uint32_t t = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
     return t;
 }
+__device__ __forceinline__ uint32_t mx4_top8(const uint4 u) {          // bfloat16, two a word
+    const uint32_t m = 0x7fff7fffu;
+    const uint32_t t = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+    return max(t << 16, t & 0xffff0000u);
+}
 
-// Eight neighbouring entries of one lane, the four lanes of a block side by side: their codes, and in `word` the four scale bytes of
-// the 128 entries of the lane's sixteen neighbours.  `v` is used up.
-__device__ __forceinline__ uint32_t mx4_quantize8(float (&v)[8], int lane, uint32_t& word) {
-    uint32_t top = mx4_top8(v);
+// The scale byte of a block whose four lanes' largest magnitudes are `top`, and in `word` the four scale bytes of the 128 entries of the
+// lane's sixteen neighbours.
+__device__ __forceinline__ uint32_t mx4_block_scale(uint32_t top, int lane, uint32_t& word) {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t s = mx4_scale_of(top);
-    const float inv = mx4_inverse(s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = s == 255u ? 0.f : v[i] * inv;
     word = s << (8 * ((lane >> 2) & 3));
     word |= __shfl_xor_sync(0xffffffffu, word, 4);
     word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    return mx4_encode8(v);
+    return s;
+}
+// Eight neighbouring entries of one lane, the four lanes of a block side by side: their codes, and `word` as above.
+__device__ __forceinline__ uint32_t mx4_quantize8(const float (&v)[8], uint32_t top, int lane, uint32_t& word) {
+    const uint32_t s = mx4_block_scale(top, lane, word);
+    const float inv = mx4_inverse(s);
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = v[i] * inv;
+    const uint32_t code = mx4_encode8(w);
+    return s == 255u ? 0u : code;
 }
 
 // Eight bfloat16 as float32.
