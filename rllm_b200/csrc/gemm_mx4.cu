@@ -51,33 +51,39 @@ template <bool GATED> __device__ __forceinline__ void gm_take(uint32_t taddr, in
 // memory, 128 bytes of each at a time (pieces of 16 bytes swizzled by the row), and leave as whole lines, eight lanes to a row.
 //   row0: the warp's first row, n0: the first column of what its threads hold, `vec`: rows of C begin at multiples of 16 bytes
 template <typename TC, int EPI> __device__ __forceinline__ void gm_give(const uint32_t (&r)[4][32], unsigned char* stage, int lane, TC* C, long long ldc,
-                                                                        int row0, int m_end, int n0, int N, bool vec, const GluForm& glu) {
+                                                                        int row0, int m_end, int n0, int N, bool vec, const Mx4Glu& glu) {
     constexpr bool GATED = EPI == GM_EPI_GATED;
     constexpr int PER = 128 / (int)sizeof(TC), PIECE = 16 / (int)sizeof(TC), OUT = GATED ? 64 : 128;
 #pragma unroll
     for (int c = 0; c < OUT / PER; ++c) {
         if (n0 + c * PER >= N) break;
+        auto pieces = [&](auto value) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float v[PIECE];
+            for (int j = 0; j < 8; ++j) {
+                float v[PIECE];
 #pragma unroll
-            for (int i = 0; i < PIECE; ++i) {
-                const int col = c * PER + j * PIECE + i;
-                const float x = __uint_as_float(r[col >> 5][col & 31]);
-                v[i] = GATED ? mx4_glu(glu, x, __uint_as_float(r[(col >> 5) + (GATED ? 2 : 0)][col & 31])) : x;
-            }
-            uint4 u;
-            if constexpr (sizeof(TC) == 4) u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-            else {
-                uint32_t w[4];
+                for (int i = 0; i < PIECE; ++i) v[i] = value(c * PER + j * PIECE + i);
+                uint4 u;
+                if constexpr (sizeof(TC) == 4) u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                else {
+                    uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+                    for (int i = 0; i < 4; ++i) {
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+                    }
+                    u = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                u = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
             }
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+        };
+        if constexpr (GATED) {
+            auto gate = [&](int col) { return __uint_as_float(r[col >> 5][col & 31]); };
+            auto up = [&](int col) { return __uint_as_float(r[(col >> 5) + 2][col & 31]); };
+            if (glu.gelu) pieces([&](int col) { return glu.template at<true>(gate(col), up(col)); });
+            else pieces([&](int col) { return glu.template at<false>(gate(col), up(col)); });
+        } else {
+            pieces([&](int col) { return __uint_as_float(r[col >> 5][col & 31]); });
         }
         __syncwarp();
         const int col = n0 + c * PER + (lane & 7) * PIECE;
@@ -291,6 +297,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         unsigned char* stage = smem + GM_STAGES * GM_STAGE_BYTES + (warp - 2) * 4096;
         const bool vec = ((uintptr_t)C & 15) == 0 && ((ldc * (long long)sizeof(TC)) & 15) == 0;
+        const Mx4Glu unit(glu);
         int local = 0;
         for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++local) {
             int e, mt, m0, m_end, n0;
@@ -306,7 +313,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             tc_fence_before();
             mbar_arrive(&acc_empty);
             if (m0 + quarter * 32 < m_end)
-                gm_give<TC, EPI>(r, stage, lane, C, ldc, m0 + quarter * 32, m_end, n0 + (GATED ? 64 : 128) * half, N, vec, glu);
+                gm_give<TC, EPI>(r, stage, lane, C, ldc, m0 + quarter * 32, m_end, n0 + (GATED ? 64 : 128) * half, N, vec, unit);
         }
     }
     __syncwarp();          // the lanes that had no role meet the elected one: the barrier below wants whole warps
@@ -504,6 +511,7 @@ gemm_mx4_pair_kernel(const __grid_constant__ GpMaps maps, TC* C, long long ldc, 
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         unsigned char* stage = smem + GP_STAGES * GP_STAGE_BYTES + (warp - 2) * 4096;
         const bool vec = ((uintptr_t)C & 15) == 0 && ((ldc * (long long)sizeof(TC)) & 15) == 0;
+        const Mx4Glu unit(glu);
         int local = 0;
         for (int tile = pair; tile < total_tiles; tile += n_pairs, ++local) {
             int e, block, m0, m_end, n0;
@@ -520,7 +528,7 @@ gemm_mx4_pair_kernel(const __grid_constant__ GpMaps maps, TC* C, long long ldc, 
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gp_leader(&acc_empty)) : "memory");
             if (m0 + quarter * 32 < m_end)
-                gm_give<TC, EPI>(r, stage, lane, C, ldc, m0 + quarter * 32, m_end, n0 + (GATED ? 64 : 128) * half, N, vec, glu);
+                gm_give<TC, EPI>(r, stage, lane, C, ldc, m0 + quarter * 32, m_end, n0 + (GATED ? 64 : 128) * half, N, vec, unit);
         }
     }
     __syncwarp();

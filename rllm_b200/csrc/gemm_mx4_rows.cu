@@ -299,6 +299,7 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
     __syncthreads();
     // NB rows of X at a column of C, from b0 in steps of `step`: the old values are all on their way before the first is used
     constexpr int NB = 8;
+    const Mx4Glu unit(glu);
     auto write = [&](int b0, int step, int col, const float (&sum)[HALVES][NB]) {
         if (col >= n || !ep_ok) return;
         TC* dst = C + (size_t)(r0 + b0) * ldc + col;
@@ -309,7 +310,7 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            float o = GATED ? mx4_glu(glu, sum[0][i], sum[HALVES - 1][i]) : sum[0][i];
+            float o = !GATED ? sum[0][i] : unit.gelu ? unit.template at<true>(sum[0][i], sum[HALVES - 1][i]) : unit.template at<false>(sum[0][i], sum[HALVES - 1][i]);
             if (EPI == GR_EPI_ACCUM) o += old[i];
             if (b0 + i * step < m) dst[(size_t)(i * step) * ldc] = from_f<TC>(o);
         }

@@ -51,52 +51,48 @@ mx4_quantize_kernel(const T* x, long long ld, int rows, int k, uint8_t* codes, u
     if (w >= n_warps) return;
     const unsigned item = w / per_row;
     const int chunks = (k + MX4_CHUNK - 1) / MX4_CHUNK, c0 = (int)(w - item * per_row) * MQ_RUNS;
-    long long src = item, row = item, scale_row = item;
-    if (SORTED) {
-        if (place) {
-            row = place[item];
-            src = item / (unsigned)top_k;
-            if (row < 0 || row >= rows) return;
-        }
-    }
     MqPart<T> part[MQ_RUNS];
-    const bool here = item < (unsigned)rows;                     // (rows behind the last one get scales of zero)
+    const bool here = SORTED || item < (unsigned)rows;           // (rows behind the last one get scales of zero)
     const int col0 = c0 * MX4_CHUNK + lane * 8, left = here ? k - col0 : 0;      // (k is a multiple of 32: a lane's eight are all in or all out)
-    const T* from = x + src * ld + col0;
+    const T* from = x + item * ld + col0;
 #pragma unroll
     for (int i = 0; i < MQ_RUNS; ++i) {
         if (i * MX4_CHUNK < left) part[i].template load<VEC>(from + i * MX4_CHUNK);
         else part[i].zero();
     }
-    if (SORTED) {
+    uint32_t code[MQ_RUNS], word[MQ_RUNS];
+#pragma unroll
+    for (int i = 0; i < MQ_RUNS; ++i) code[i] = part[i].codes(lane, word[i]);
+    auto store = [&](long long row, long long scale_row) {
+        uint8_t* code_to = codes + row * (long long)(k >> 1) + (col0 >> 1);
+        uint8_t* scale_to = scales + mx4_scale_at(scale_row, (long long)c0 * 8 + (lane >> 4) * 4, 2ll * chunks);
+#pragma unroll
+        for (int i = 0; i < MQ_RUNS; ++i) {
+            if (c0 + i >= chunks) break;
+            if (i * MX4_CHUNK < left) *reinterpret_cast<uint32_t*>(code_to + i * (MX4_CHUNK / 2)) = code[i];
+            if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scale_to + i * 2 * MX4_ATOM) = word[i];
+        }
+    };
+    if (!SORTED) {
+        store(item, item);
+        return;
+    }
+    for (int j = 0; j < top_k; ++j) {                            // a token's row goes to the places of its pairs
+        const int row = place ? place[(long long)item * top_k + j] : (int)item;
+        if (row < 0 || row >= rows) continue;
         // the row's expert is the first that ends behind it; its rows begin behind the row tiles of the experts before
         int before = 0, tiles = 0;
-        for (int e = lane; e < E; e += 32) {
-            const int end = offsets[e + 1];
-            if (end <= row) {
-                ++before;
-                tiles += (end - offsets[e] + 127) >> 7;
-            }
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + lane, end = e < E ? offsets[e + 1] : 0x7fffffff;
+            const unsigned past = __ballot_sync(0xffffffffu, end <= row);
+            if (past == 0) break;
+            before += __popc(past);
+            tiles += __reduce_add_sync(0xffffffffu, end <= row ? (end - offsets[e] + 127) >> 7 : 0);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            before += __shfl_xor_sync(0xffffffffu, before, o);
-            tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-        }
-        if (before >= E) return;
-        scale_row = (long long)tiles * 128 + (row - offsets[before]);
+        if (before >= E) continue;
+        const long long scale_row = (long long)tiles * 128 + (row - offsets[before]);
         // (offsets that do not rise from 0 to the number of rows: nothing outside the scales is written)
-        if (scale_row < 0 || scale_row >= ((long long)((rows + 127) >> 7) + E) * 128) return;
-    }
-    uint8_t* code_to = codes + row * (long long)(k >> 1) + (col0 >> 1);
-    uint8_t* scale_to = scales + mx4_scale_at(scale_row, (long long)c0 * 8 + (lane >> 4) * 4, 2ll * chunks);
-#pragma unroll
-    for (int i = 0; i < MQ_RUNS; ++i) {
-        if (c0 + i >= chunks) break;
-        uint32_t word;
-        const uint32_t code = part[i].codes(lane, word);
-        if (i * MX4_CHUNK < left) *reinterpret_cast<uint32_t*>(code_to + i * (MX4_CHUNK / 2)) = code;
-        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scale_to + i * 2 * MX4_ATOM) = word;
+        if (scale_row >= 0 && scale_row < ((long long)((rows + 127) >> 7) + E) * 128) store(row, scale_row);
     }
 }
 
@@ -155,11 +151,12 @@ static unsigned mq_warps(long long rows, int k, unsigned& per_row) {
     return n < 0xfffffff0ll ? (unsigned)n : 0u;
 }
 
+// items: rows to read, with pad those whose scales are written
 template <typename T, bool VEC>
-static int mx4_launch(const T* x, long long ld, int rows, int k, uint8_t* codes, uint8_t* scales, int pad_rows, const int* offsets,
+static int mx4_launch(const T* x, long long ld, int rows, int k, uint8_t* codes, uint8_t* scales, int items, const int* offsets,
                       const int* place, int E, int top_k, cudaStream_t stream) {
     unsigned per_row;
-    const unsigned n = mq_warps(pad_rows, k, per_row);
+    const unsigned n = mq_warps(items, k, per_row);
     if (!n) return (int)cudaErrorInvalidValue;
     const dim3 grid(n / 4 + (n % 4 != 0));
     if (offsets)
@@ -175,14 +172,14 @@ static int mx4_launch(const T* x, long long ld, int rows, int k, uint8_t* codes,
 RLLM_API int rllm_mx4_quantize(const void* x, void* codes, void* scales, const int* offsets, const int* place, long long ld, int dt,
                                int rows, int k, int pad, int E, int top_k, cudaStream_t stream) {
     if (rows <= 0 || k <= 0) return 0;
-    if ((k % MX4_BLOCK) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15) || (offsets && (E <= 0 || pad)) || (place && top_k <= 0) ||
+    if ((k % MX4_BLOCK) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15) || (offsets && (E <= 0 || pad)) || (place && (top_k <= 0 || rows % top_k)) ||
         (place && !offsets) || rows > 0x7fffff00)
         return (int)cudaErrorInvalidValue;
-    const int pad_rows = pad ? (rows + 127) / 128 * 128 : rows;
+    const int items = pad ? (rows + 127) / 128 * 128 : place ? rows / top_k : rows;
     const int esize = dt == RLLM_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)x & 15) == 0 && (ld * esize) % 16 == 0;
 #define MX4_Q(T, VEC) \
-    return mx4_launch<T, VEC>((const T*)x, ld, rows, k, (uint8_t*)codes, (uint8_t*)scales, pad_rows, offsets, place, E, top_k, stream)
+    return mx4_launch<T, VEC>((const T*)x, ld, rows, k, (uint8_t*)codes, (uint8_t*)scales, items, offsets, place, E, place ? top_k : 1, stream)
     if (dt == RLLM_F32) { if (vec) { MX4_Q(float, true); } MX4_Q(float, false); }
     if (vec) { MX4_Q(bf16, true); }
     MX4_Q(bf16, false);
