@@ -384,7 +384,7 @@ RLLM_API int rllm_mx4_quantize(const void* x, void* codes, void* scales, const i
 
 // X: rows of K entries, ldx apart, float32 or bfloat16; C [m, n].  W: codes [n, K / 2] and scales, gated: gate and up matrix of n rows each,
 // experts: E times that.  bn: rows of X to a CTA.  16: they are quantised by the product itself (16-byte aligned rows); 32, 64 (all rows in
-// one chunk) and 128: by a launch ahead of it, into `work` (codes, and from the next multiple of 1,024 bytes the scales).  splits: 1, 2, 4
+// one chunk) and 128 (not gated): by a launch ahead of it, into `work` (codes, and from the next multiple of 1,024 bytes the scales).  splits: 1, 2, 4
 // or 8 CTAs (gated: pairs, up to 4) share a tile's K.  offsets, place, top_k: see the top (bn 16; place: X holds m / top_k rows).  ahead: W is
 // settled and may be read before the kernels before have ended.  epilogue 0 store, 1 add into a float32 C, 2 gated (GluForm).  Returns 0, a
 // cudaError_t or 30000 + CUresult.
@@ -423,11 +423,13 @@ RLLM_API int rllm_mx4_rows_product(const void* X, const int* offsets, const int*
         if (bn == 16) { GR_GO(16, 3, 4, 3, EPI, TC, bf16); }                                                    \
         if (bn == 32) { GR_GO(32, 3, 4, 3, EPI, TC, uint8_t); }                                                 \
         if (bn == 64) { GR_GO(64, 4, 8, 2, EPI, TC, uint8_t); }                                                 \
-        if (bn == 128) { GR_GO(128, 3, 8, 2, EPI, TC, uint8_t); }                                               \
     }
-    if (epilogue == GR_EPI_STORE) { if (c_dtype == RLLM_F32) GR_BN(GR_EPI_STORE, float) else GR_BN(GR_EPI_STORE, bf16) }
-    if (epilogue == GR_EPI_ACCUM) GR_BN(GR_EPI_ACCUM, float)
+#define GR_128(EPI, TC) if (bn == 128) { GR_GO(128, 3, 8, 2, EPI, TC, uint8_t); }
+    if (epilogue == GR_EPI_STORE && c_dtype == RLLM_F32) { GR_BN(GR_EPI_STORE, float) GR_128(GR_EPI_STORE, float) }
+    if (epilogue == GR_EPI_STORE && c_dtype != RLLM_F32) { GR_BN(GR_EPI_STORE, bf16) GR_128(GR_EPI_STORE, bf16) }
+    if (epilogue == GR_EPI_ACCUM) { GR_BN(GR_EPI_ACCUM, float) GR_128(GR_EPI_ACCUM, float) }
     if (gated) { if (c_dtype == RLLM_F32) GR_BN(GR_EPI_GATED, float) else GR_BN(GR_EPI_GATED, bf16) }
+#undef GR_128
 #undef GR_BN
 #undef GR_GO
     return (int)cudaErrorInvalidValue;

@@ -2106,18 +2106,20 @@ def mx4_quantize(x):
     return Mx4Matrix.__new__(Mx4Matrix)._set(codes, scales, (*lead, n, k))
 
 
-def mx4_row_splits(tiles: int, k: int, bn: int, gated: bool, n_sm: int = 148) -> int:
+def mx4_row_splits(tiles: int, k: int, bn: int, gated: bool, experts: bool = False, n_sm: int = 148) -> int:
     """CTAs that share the K of a tile of 128 weight rows in the product of few rows; tiles: with gate and up, experts and chunks of rows
     counted apart.  A CTA keeps a least number of stages of 256 entries, below which the exchange of the sums costs more than it saves, and
-    all CTAs run at once (three an SM with bn 16 and 32, two with 64 and 128).  us with 1 / 2 / 4 / 8:
+    all CTAs run at once (three an SM with bn 16 and 32, two with 64 and 128; experts: two, the last of them seldom have rows).  us with 1 / 2 /
+    4 / 8:
         bn 16,  8 rows:   4,096 x 4,096 11.9 / 8.0 / 7.4 / 7.1, 4,096 x 1,024 4.4 / 4.5 / 4.8, 4,096 x 12,288 30.8 / 17.3 / 12.4 / 10.6,
-                          gated 2 x 12,288 x 4,096 17.0 / 12.7 / 21.6
-        bn 32, 16 rows:   4,096 x 4,096 8.4 / 8.0 / 7.7 / 8.8, 1,000 x 2,080 6.0 / 6.7 / 6.6, gated 2 x 12,288 x 4,096 15.1 / 13.9 / 20.5
-        bn 64, 64 rows:   4,096 x 4,096 8.0 / 9.0 / 8.5 / 13.2, 4,096 x 12,288 16.9 / 13.8 / 12.4 / 15.4, gated 2 x 1,536 x 2,048 8.9 / 7.8 / 8.3
-        bn 128, 128 rows: 4,096 x 4,096 9.0 / 11.0 / 11.4, 4,096 x 12,288 23.4 / 19.9 / 17.8, gated 2 x 768 x 2,048 13.0 / 10.8 / 10.4"""
+                          gated 2 x 12,288 x 4,096 16.1 / 12.4 / 21.3, 2 x 1,536 x 2,048 8.2 / 6.2 / 5.8
+        bn 32, 16 rows:   4,096 x 4,096 8.4 / 8.0 / 7.7 / 8.8, 1,000 x 2,080 6.0 / 6.7 / 6.6, gated 2 x 12,288 x 4,096 14.8 / 14.1 / 20.6
+        bn 64, 64 rows:   4,096 x 4,096 8.0 / 9.0 / 8.5 / 13.2, 4,096 x 12,288 16.9 / 13.8 / 12.4 / 15.4, gated 2 x 1,536 x 2,048 8.6 / 7.7 / 8.2
+        bn 128, 128 rows: 4,096 x 4,096 9.0 / 11.0 / 11.4, 4,096 x 12,288 23.4 / 19.9 / 17.8
+        experts, 8 tokens to 4 each: of 16, 2 x 768 x 2,048 9.3 / 10.1, of 4, 2 x 1,536 x 4,096 (2 each) 13.8 / 10.1"""
     chunks = -(-k // 256)
     if bn == 16:
-        least, most = 2, 3 * n_sm
+        least, most = 2, (2 if experts else 3) * n_sm
     elif gated:
         least, most = 4, 3 * n_sm if bn == 32 else n_sm
     elif bn == 32:
@@ -2135,31 +2137,31 @@ def mx4_few_rows(rows: int, n: int, k: int, gated: bool, own: bool, experts: int
     """(rows of x to a CTA, CTAs that share K) for the product of few rows (gemm_mx4_rows.cu), or None: the one of many rows (gemm_mx4.cu).
     own: the rows lie as the kernel that quantises them itself (bn 16) reads them; experts: of sorted rows (0: none).
     bn 16 is one launch, but every CTA quantises its part of the rows again: up to 8 rows it is as fast as a launch ahead of it (gated
-    8 x 12,288 x 4,096: 12.7 us against 13.9), beyond that with small matrices only (16 x 12,288 x 4,096 gated: 16.6 against 13.9; 16 x 4,096
-    x 1,024: 4.9 against 4.3, where the second launch costs the host more than that).  Sorted rows: while experts have few each (32 pairs of 16
-    experts of 768 x 2,048: 10 us against 18; 400 pairs: 18.8 against 14.7).
+    8 x 12,288 x 4,096: 12.4 us against 13.6), beyond that with small matrices only (16 x 12,288 x 4,096 gated: 15.9 against 14.1; 16 x 4,096
+    x 1,024: 4.9 against 4.3, where the second launch costs the host more than that).  Sorted rows: while experts have few each (of 16 experts of
+    768 x 2,048: 32 pairs 9.3 us against 13.5, 128 pairs 12.2 against 12.6, 256 pairs 14.2 against 12.9).
     bn 128 against tiles of 128 x 256, one an SM: as long as its CTAs all run at once, two an SM (512 x 4,096 x 4,096 12.0 us against 13.7,
-    300 x 1,000 x 2,080 8.0 against 10.8, 1,024 x 6,144 x 4,096 21.7 against 22.0); gated, where it takes twice the CTAs, half of that a
-    quarter (256 x 1,536 x 2,048 11.3 against 12.6, 512 rows 14.2 against 13.1)."""
+    300 x 1,000 x 2,080 8.0 against 10.8, 1,024 x 6,144 x 4,096 21.7 against 22.0); not for gated products, where it takes twice the CTAs and
+    exchanges their sums (100 x 1,536 x 2,048 9.3 against 8.5)."""
     tiles = -(-n // 128) * (2 if gated else 1)
     if experts:
         if not own or rows > min(256, 8 * experts):
             return None
-        return 16, mx4_row_splits(tiles * min(experts, rows), k, 16, gated, n_sm)
+        return 16, mx4_row_splits(tiles * min(experts, rows), k, 16, gated, True, n_sm)
     if own and rows <= 16 and (rows <= 8 or tiles * k <= 1 << 16):
-        return 16, mx4_row_splits(tiles, k, 16, gated, n_sm)
+        return 16, mx4_row_splits(tiles, k, 16, gated, False, n_sm)
     bn = 32 if rows <= 32 else 64 if rows <= 64 else 128
     tiles *= -(-rows // bn)
-    if bn == 128 and tiles > (n_sm // 2 if gated else 2 * n_sm):
+    if bn == 128 and (gated or tiles > 2 * n_sm):
         return None
-    return bn, mx4_row_splits(tiles, k, bn, gated, n_sm)
+    return bn, mx4_row_splits(tiles, k, bn, gated, False, n_sm)
 
 
 def mx4_pairs(rows: int, n: int, k: int, gated: bool, experts: int = 0, n_sm: int = 148) -> bool:
     """Whether the product of many rows takes two SMs to a tile of 256 x 256 (a stage of 256 entries 0.38 us, a tile 1.6 us beside its
     stages) or one to a tile of 128 x 256 (0.41 us): whichever needs less time for its waves.  us, one / two: 4,096 x 12,288 x 2,048 rows 61.1 /
-    54.6, 4,096 x 4,096: 512 rows 13.7 / 14.2, 2,048 rows 24.1 / 23.6; gated 2 x 12,288 x 4,096: 1,024 rows 54.2 / 49.7, 2,048 rows 93.5 / 87.3;
-    gated 2 x 1,536 x 2,048: 2,048 rows 22.7 / 24.6.  Routed experts seldom fill tiles of 256 rows (4,000 pairs of 16: 18.0 / 21.3)."""
+    54.6, 4,096 x 4,096: 512 rows 13.7 / 14.2, 2,048 rows 24.1 / 23.6; gated 2 x 12,288 x 4,096: 1,024 rows 53.1 / 49.0, 2,048 rows 91.2 / 85.9;
+    gated 2 x 1,536 x 2,048: 2,048 rows 14.1 / 17.7.  Routed experts seldom fill tiles of 256 rows (4,000 pairs of 16: 17.6 / 20.5)."""
     if experts:
         return False
     cols, stages = -(-n // (128 if gated else 256)), -(-k // 256)
