@@ -86,28 +86,29 @@ template <typename TC, int EPI> __device__ __forceinline__ void gm_give(const ui
             pieces([&](int col) { return __uint_as_float(r[col >> 5][col & 31]); });
         }
         __syncwarp();
-        const int col = n0 + c * PER + (lane & 7) * PIECE;
+        if (vec && n0 + (c + 1) * PER <= N) {
+            const int col = n0 + c * PER + (lane & 7) * PIECE;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = i * 4 + (lane >> 3), gm = row0 + row;
-            uint4 u = *reinterpret_cast<const uint4*>(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
-            if (gm < m_end && col < N) {
-                TC* dst = C + (size_t)gm * ldc + col;
-                if (vec && col + PIECE <= N) {
-                    if constexpr (EPI == GM_EPI_ACCUM) {
-                        const float4 o = *reinterpret_cast<const float4*>(dst);
-                        u = make_uint4(__float_as_uint(__uint_as_float(u.x) + o.x), __float_as_uint(__uint_as_float(u.y) + o.y),
-                                       __float_as_uint(__uint_as_float(u.z) + o.z), __float_as_uint(__uint_as_float(u.w) + o.w));
+            for (int i = 0; i < 8; ++i) {
+                const int row = i * 4 + (lane >> 3), gm = row0 + row;
+                const uint4 u = *reinterpret_cast<const uint4*>(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+                if (gm < m_end) {
+                    TC* dst = C + (size_t)gm * ldc + col;
+                    if constexpr (EPI == GM_EPI_ACCUM) add_to4(dst, u);
+                    else *reinterpret_cast<uint4*>(dst) = u;
+                }
+            }
+        } else {                                     // rows at any address, columns that end inside: a row at a time, neighbouring lanes side by side
+            for (int row = 0; row < 32 && row0 + row < m_end; ++row) {
+                TC* dst = C + (size_t)(row0 + row) * ldc + n0 + c * PER;
+#pragma unroll
+                for (int h = 0; h < PER / 32; ++h) {
+                    const int at = h * 32 + lane, piece = at / PIECE;
+                    const TC v = *reinterpret_cast<const TC*>(stage + row * 128 + ((piece ^ (row & 7)) << 4) + (at & (PIECE - 1)) * (int)sizeof(TC));
+                    if (n0 + c * PER + at < N) {
+                        if constexpr (EPI == GM_EPI_ACCUM) add_to(dst + at, v);
+                        else dst[at] = v;
                     }
-                    *reinterpret_cast<uint4*>(dst) = u;
-                } else {
-                    const TC* from = reinterpret_cast<const TC*>(&u);
-#pragma unroll
-                    for (int k = 0; k < PIECE; ++k)
-                        if (col + k < N) {
-                            if constexpr (EPI == GM_EPI_ACCUM) dst[k] += from[k];
-                            else dst[k] = from[k];
-                        }
                 }
             }
         }

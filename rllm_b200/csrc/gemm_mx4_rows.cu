@@ -297,22 +297,19 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
     __syncwarp();          // the lanes that had no role meet the elected one: the barriers below want whole warps
     tc_fence_before();
     __syncthreads();
-    // NB rows of X at a column of C, from b0 in steps of `step`: the old values are all on their way before the first is used
+    // NB rows of X at a column of C, from b0 in steps of `step`
     constexpr int NB = 8;
     const Mx4Glu unit(glu);
     auto write = [&](int b0, int step, int col, const float (&sum)[HALVES][NB]) {
         if (col >= n || !ep_ok) return;
         TC* dst = C + (size_t)(r0 + b0) * ldc + col;
-        float old[NB];
-        if (EPI == GR_EPI_ACCUM) {
-#pragma unroll
-            for (int i = 0; i < NB; ++i) old[i] = b0 + i * step < m ? to_f<TC>(dst[(size_t)(i * step) * ldc]) : 0.f;
-        }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            float o = !GATED ? sum[0][i] : unit.gelu ? unit.template at<true>(sum[0][i], sum[HALVES - 1][i]) : unit.template at<false>(sum[0][i], sum[HALVES - 1][i]);
-            if (EPI == GR_EPI_ACCUM) o += old[i];
-            if (b0 + i * step < m) dst[(size_t)(i * step) * ldc] = from_f<TC>(o);
+            const float o = !GATED ? sum[0][i] : unit.gelu ? unit.template at<true>(sum[0][i], sum[HALVES - 1][i]) : unit.template at<false>(sum[0][i], sum[HALVES - 1][i]);
+            if (b0 + i * step < m) {
+                if constexpr (EPI == GR_EPI_ACCUM) add_to(dst + (size_t)(i * step) * ldc, o);
+                else dst[(size_t)(i * step) * ldc] = from_f<TC>(o);
+            }
         }
     };
     if (ranks > 1) {

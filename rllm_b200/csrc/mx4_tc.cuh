@@ -105,6 +105,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* r) {
         : "r"(taddr) : "memory");
 }
 
+// C += v where the sum is made, in L2: nobody waits for the old value (an element gets one addition a launch, so the result does not depend on any
+// order; a sum below 2^-126 becomes zero).  2,048 x 4,096 x 4,096: 49 us with loads and stores, 26 with these, 25 where C is only written.
+__device__ __forceinline__ void add_to(float* p, float v) { asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory"); }
+__device__ __forceinline__ void add_to4(float* p, const uint4 v) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                 ::"l"(p), "f"(__uint_as_float(v.x)), "f"(__uint_as_float(v.y)), "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w)) : "memory");
+}
+
 // The gated unit of common.cuh's GluForm with the fast division, 2 ulp where the denominator is below 2^126; beyond it the result is 0 either way.
 // What the form asks is decided once: no clamp is a clamp at infinity, and the tanh form of gelu (alpha 0) a function of its own.  The
 // clamps leave a NaN what it is.  (With the questions asked for every element a tile of 128 x 256 took 1.9 us longer to end.)

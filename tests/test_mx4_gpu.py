@@ -349,6 +349,74 @@ def test_feed_forward_chain():
     ops().check_device_errors()
 
 
+@pytest.mark.parametrize("m", [3, 70, 200])
+def test_offsets_beyond_32_bits(m, many):
+    """Rows in and out 2^25 and more entries apart, so that the last ones lie beyond 2^31 entries; what lies beside them stays."""
+    n, k, apart = 136, 320, (1 << 31) // (m - 1) + 64
+    apart -= apart % 8
+    x = torch.empty((m - 1) * apart + k, dtype=torch.bfloat16, device=DEV).as_strided((m, k), (apart, 1))
+    x.copy_(rnd(m, k, seed=1))
+    w, values = weight(n, k, seed=2)
+    out = torch.zeros((m - 1) * apart + n, device=DEV).as_strided((m, n), (apart, 1))
+    want, size = plain.product(plain.quantize(x.contiguous())[2], values)
+    plain.near(ops().linear(x, w, out=out), want, plain.product_slack(size, k))
+    assert float(out[0].abs().sum()) == float(out.as_strided((apart,), (1,)).abs().sum())
+    ops().linear(x, w, out=out, accumulate=True)
+    plain.near(out, 2 * want, 2 * plain.product_slack(size, k))
+    q = ops().mx4_quantize(x)
+    assert torch.equal(q.dequantize().double(), plain.quantize(x.contiguous())[2])
+
+
+@pytest.mark.parametrize("m", [1, 40, 129])
+def test_weights_beyond_32_bits(m):
+    """Codes of more than 2^32 bytes: the last columns come from the last rows."""
+    n, k, tail = (1 << 20) + 200, 8256, 300
+    codes = torch.zeros(n, k // 2, dtype=torch.uint8, device=DEV)
+    scales = torch.full(ops().mx4_scale_shape(n, k), 127, dtype=torch.uint8, device=DEV)
+    w = ops().Mx4Matrix(codes, scales)
+    c = torch.randint(0, 16, (tail, k), generator=torch.Generator().manual_seed(1)).to(DEV)
+    codes[-tail:] = plain.pack(c)
+    x = rnd(m, k, seed=2, dtype=torch.bfloat16)
+    values = plain.dequantize(c, torch.full((tail, k // 32), 127, device=DEV))
+    want, size = plain.product(plain.quantize(x)[2], values)
+    out = ops().linear(x, w, out_dtype=torch.float32)
+    plain.near(out[:, -tail:], want, plain.product_slack(size, k))
+    assert float(out[:, :-tail].abs().max()) == 0.0
+    del out
+    if m == 1:
+        got = w.dequantize(torch.bfloat16)
+        assert torch.equal(got[-tail:].double(), values) and not bool(got[:-tail].any())
+        again = ops().mx4_quantize(got)                       # 17 GB in, rows beyond 2^32 entries
+        assert torch.equal(again.dequantize(torch.bfloat16)[-tail:], got[-tail:])
+
+
+def test_two_threads_at_once():
+    """Products called from two threads, each on a stream of its own."""
+    import threading
+    w, values = weight(512, 768, seed=1)
+    g, _ = weight(2, 320, 768, seed=2)
+    xs = [rnd(m, 768, seed=m, dtype=torch.bfloat16) for m in (3, 90)]
+    want = [(ops().linear(x, w), ops().gate_up_swiglu(x, g, torch.empty(x.shape[0], 320, dtype=torch.bfloat16, device=DEV))) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def go(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(200):
+                a = ops().linear(xs[i], w)
+                b = ops().gate_up_swiglu(xs[i], g, torch.empty(xs[i].shape[0], 320, dtype=torch.bfloat16, device=DEV))
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=go, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    ops().check_device_errors()
+
+
 # ---------------------------------------------------------------- refusals
 
 def test_refusals():
