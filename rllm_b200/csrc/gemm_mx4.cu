@@ -10,7 +10,10 @@
 //   * every stage has tensor-memory columns of its own for its scales: they are overwritten only when the products that read them
 //     have released the stage;
 //   * the accumulator takes 256 of the 512 columns, so there is one: eight epilogue warps take it into registers (128 a thread) and hand it
-//     back before they convert and store.
+//     back before they convert and store; between two tiles the pipe waits 1.1 to 1.6 us for that.
+// A stage's four products need 512 cycles and the copies of its scales, which queue in the same pipe, about 190 more: 0.41 us a stage at the clocks
+// under load (0.38 in pairs, below).  Gated 256 x 1,536 x 2,048: 8.8 us with the quantisation of the rows ahead of it; 4,000 rows of 16 experts, 2 x 768 x
+// 2,048: 15.5 us of 19.9.  Where K is short the tile's end decides: its rows leave as whole lines (gm_give).
 // The rows of A may be sorted by expert (offsets int32 [E + 1] on the device): expert e's rows form row tiles of their own, counted by
 // every CTA itself, whose scales lie in the same order (rllm_mx4_quantize); its matrix is number e of the stack B.
 // The gated product: B is a stack of gate and up matrices in turn; a tile holds 128 gate rows and the 128 up rows of the same index.
@@ -326,8 +329,8 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 // ---------------------------------------------------------------- two SMs to a tile
 // The same product by pairs of CTAs (tcgen05.mma.cta_group::2, a cluster of two along x): a pair computes 256 x 256, each CTA stages its own
 // 128 rows of A and its half of the tile of B, and holds the accumulator of its rows.  A stage of 256 entries along K is then 35 KB a CTA where the
-// kernel above fills 51, and that is what bounds it: its 51 KB a stage came at 41 bytes a clock and SM (2,048 x 4,096 x 12,288), the same with
-// three quarters of the tensor instructions left out.
+// kernel above fills 51, and five stages fit.  2,048 x 4,096 x 12,288: 40 us behind 12 of quantisation, 5.2 PFLOP/s (61 us together with one SM a tile, 52
+// with two); gated 2,048 x 2 x 12,288 x 4,096: 80 us, 5.2 PFLOP/s.
 //   * the scales of A belong to each CTA's own rows; those of B are needed whole by both, so each loads both blocks;
 //   * the loads of both CTAs complete on the leader's barrier; a plain bulk copy cannot signal the peer's barrier, so the scales, too, come by
 //     tensor loads, from a map of lines of 1,024 bytes;

