@@ -10,9 +10,9 @@
 //   * every stage has tensor-memory columns of its own for its scales: they are overwritten only when the products that read them
 //     have released the stage;
 //   * the accumulator takes 256 of the 512 columns, so there is one: eight epilogue warps take it into registers (128 a thread) and hand it
-//     back before they convert and store; between two tiles the pipe waits 1.1 to 1.6 us for that.
-// A stage's four products need 512 cycles and the copies of its scales, which queue in the same pipe, about 190 more: 0.41 us a stage at the clocks
-// under load (0.38 in pairs, below).  Gated 256 x 1,536 x 2,048: 8.8 us with the quantisation of the rows ahead of it; 4,000 rows of 16 experts, 2 x 768 x
+//     back before they convert and store (handed back before it was read, a launch took as long: the stores cost, not the hand-over).
+// A stage's four products need 512 cycles: 0.27 us at 1.9 GHz, 0.31 at the 1.68 GHz that long launches run at under the power cap; a stage takes 0.41 us
+// (in pairs, below, 0.31 to 0.38).  The copies of the scales are not what is missing: with half of them left out it took as long.  Gated 256 x 1,536 x 2,048: 8.8 us with the quantisation of the rows ahead of it; 4,000 rows of 16 experts, 2 x 768 x
 // 2,048: 15.5 us of 19.9.  Where K is short the tile's end decides: its rows leave as whole lines (gm_give).
 // The rows of A may be sorted by expert (offsets int32 [E + 1] on the device): expert e's rows form row tiles of their own, counted by
 // every CTA itself, whose scales lie in the same order (rllm_mx4_quantize); its matrix is number e of the stack B.

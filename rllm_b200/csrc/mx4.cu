@@ -74,11 +74,8 @@ mx4_quantize_kernel(const T* x, long long ld, int rows, int k, uint8_t* codes, u
             if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scale_to + i * 2 * MX4_ATOM) = word[i];
         }
     };
-    if (!SORTED) {
-        store(item, item);
-        return;
-    }
-    for (int j = 0; j < top_k; ++j) {                            // a token's row goes to the places of its pairs
+    if constexpr (!SORTED) store(item, item);
+    else for (int j = 0; j < top_k; ++j) {                       // a token's row goes to the places of its pairs
         const int row = place ? place[(long long)item * top_k + j] : (int)item;
         if (row < 0 || row >= rows) continue;
         // the row's expert is the first that ends behind it; its rows begin behind the row tiles of the experts before

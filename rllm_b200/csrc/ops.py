@@ -2158,9 +2158,8 @@ def mx4_few_rows(rows: int, n: int, k: int, gated: bool, own: bool, experts: int
 
 
 def mx4_pairs(rows: int, n: int, k: int, gated: bool, experts: int = 0, n_sm: int = 148) -> bool:
-    """Whether the product of many rows takes two SMs to a tile of 256 x 256 (a stage of 256 entries 0.38 us, a tile 1.6 us beside its
-    stages) or one to a tile of 128 x 256 (0.41 us): whichever needs less time for its waves.  us, one / two: 4,096 x 12,288 x 2,048 rows 61.1 /
-    54.6, 4,096 x 4,096: 512 rows 13.7 / 14.2, 2,048 rows 24.1 / 23.6; gated 2 x 12,288 x 4,096: 1,024 rows 53.1 / 49.0, 2,048 rows 91.2 / 85.9;
+    """Whether the product of many rows takes two SMs to a tile of 256 x 256 (a stage of 256 entries 0.38 us, a tile 1.6 us for its
+    outputs) or one to a tile of 128 x 256 (0.41 us): whichever needs less time for its waves.  us, one / two: 4,096 x 12,288 x 2,048 rows 61.1 / 54.6, 4,096 x 4,096: 512 rows 13.7 / 14.2, 2,048 rows 24.1 / 23.6; gated 2 x 12,288 x 4,096: 1,024 rows 53.1 / 49.0, 2,048 rows 91.2 / 85.9;
     gated 2 x 1,536 x 2,048: 2,048 rows 14.1 / 17.7.  Routed experts seldom fill tiles of 256 rows (4,000 pairs of 16: 17.6 / 20.5)."""
     if experts:
         return False
@@ -2246,7 +2245,10 @@ def _mx4_experts(experts, rows, offsets, place, who):
     if not 0 < experts <= MX4_MAX_EXPERTS:
         raise KernelError(f"{who}: {experts} experts (1 to {MX4_MAX_EXPERTS})")
     for name, t, size in (("offsets", offsets, experts + 1), ("place", place, rows)):
-        if t is not None:
+        if t is None:
+            if size or name == "offsets":
+                raise KernelError(f"{who}: {name} is missing")
+        else:
             _mx4_current(t)
             if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != size:
                 raise KernelError(f"{who}: {name} is int32 [{size}]")

@@ -38,6 +38,28 @@ def test_refusals():
             call()
 
 
+def test_refusals_of_experts():
+    """Sorted rows need their order: without it the products would take all rows for those of one matrix."""
+    up = ops.mx4_scale_shape(4, 64)
+    w_up = ops.Mx4Matrix(torch.zeros(3, 2, 4, 32, dtype=torch.uint8), torch.zeros(3, 2, *up, dtype=torch.uint8))
+    w_down = ops.Mx4Matrix(torch.zeros(3, 4, 32, dtype=torch.uint8), torch.zeros(3, *up, dtype=torch.uint8))
+    h, act = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(4, 4, dtype=torch.bfloat16)
+    place = torch.arange(4, dtype=torch.int32)
+    for call in (lambda: ops.mx4_experts_up(h, w_up, None, place, act), lambda: ops.mx4_experts_up(h, w_up, None, None, act),
+                 lambda: ops.mx4_experts_down(torch.zeros(4, 64, dtype=torch.bfloat16), w_down, None, act)):
+        with pytest.raises(ops.KernelError, match="offsets is missing"):
+            call()
+
+
+def test_refusal_of_unplaced_rows(monkeypatch):
+    monkeypatch.setattr(ops, "_mx4_current", lambda *t: None)               # (as on a GPU)
+    up = ops.mx4_scale_shape(4, 64)
+    w = ops.Mx4Matrix(torch.zeros(3, 2, 4, 32, dtype=torch.uint8), torch.zeros(3, 2, *up, dtype=torch.uint8))
+    act, offsets = torch.zeros(4, 4, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ops.KernelError, match="place is missing"):
+        ops.mx4_experts_up(torch.zeros(2, 64, dtype=torch.bfloat16), w, offsets, None, act)
+
+
 def test_plain_rounding():
     """The oracle itself: ties to the even code, at most 6, the scale of a block."""
     x = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9, -0.25, -0.75, -5.0, 4.0] + [0.0] * 20)
