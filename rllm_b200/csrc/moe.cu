@@ -608,7 +608,10 @@ moe_sort_kernel(const int* __restrict__ idx, int n_pairs, int E, int* offsets, i
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     for (int e = tid; e <= E; e += blockDim.x) s_count[e] = 0;
     __syncthreads();
-    for (int p = tid; p < n_pairs; p += blockDim.x) atomicAdd(&s_count[idx[p]], 1);
+    for (int p = tid; p < n_pairs; p += blockDim.x) {
+        const int e = idx[p];
+        if (e >= 0 && e < E) atomicAdd(&s_count[e], 1);      // (a pair of no expert: no place)
+    }
     __syncthreads();
     if (warp == 0) {                                       // exclusive prefix sum over the experts, 32 at a time
         int run = 0;
@@ -640,11 +643,15 @@ moe_sort_kernel(const int* __restrict__ idx, int n_pairs, int E, int* offsets, i
     }
 }
 
-// Up to MOE_SORT_E experts: one block whose 32 warps each take a 32nd of the pairs.  Twice through them, 32 at a time, the lanes that name the
-// same expert found by a ballot for each bit of its number (match.any takes a turn for every expert named): first the counts of every warp,
-// then, from what the experts and the warps before have, the places.  The same order as above (4,000 pairs of 16 experts: 9.9 us there, where a
-// warp walks all pairs for one expert, 5.6 here).
+// Up to MOE_SORT_E experts: a block, or a cluster of them, whose warps each take their share of the pairs.  Twice through them, 32 at a time, the lanes
+// that name the same expert found by a ballot for each bit of its number (match.any takes a turn for every expert named): first the counts of
+// every warp, then, from what the experts, the blocks and the warps before have, the places.  The same order as above, where every block counts all
+// pairs and every warp walks over all of them: with few pairs that is less to do, with many the walk is what it takes.  us, above / a block / a
+// cluster of 8 (its blocks wait for one another: a microsecond): 32 pairs of 16 experts 1.6 / 2.2 / 3.0, 256 of 256 2.3 / 3.0 / 4.3, 512 of 128
+// 3.0 / 2.7 / 3.8, 2,048 of 128 6.8 / 4.3 / 4.5, 4,000 of 16 8.3 / 5.3 / 3.9, 16,384 of 128 39.9 / 19.2 / 5.6, 65,536 of 128 178 / 70 / 11.4.
 #define MOE_SORT_E 256
+#define MOE_SORT_FEW 256                                     // pairs up to which the kernel above takes them,
+#define MOE_SORT_ONE 2048                                    // and one block
 __device__ __forceinline__ unsigned moe_same(int e, int bits) {
     unsigned same = 0xffffffffu;
     for (int b = 0; b < bits; ++b) {
@@ -653,25 +660,42 @@ __device__ __forceinline__ unsigned moe_same(int e, int bits) {
     }
     return same;
 }
-__global__ void __launch_bounds__(1024)
+template <int CTAS> __global__ void __launch_bounds__(1024)
 moe_sort_few_kernel(const int* idx, int n_pairs, int E, int* offsets, int* place) {
     __shared__ int s_count[32][MOE_SORT_E];
+    __shared__ int s_block[MOE_SORT_E];
     __shared__ int s_first[MOE_SORT_E + 1];
     pdl_wait();
     pdl_launch_dependents();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int per = ((n_pairs + 31) / 32 + 31) & ~31, first = warp * per, last = min(n_pairs, first + per);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = CTAS > 1 ? (int)blockIdx.x : 0;
+    const int per = ((n_pairs + 32 * CTAS - 1) / (32 * CTAS) + 31) & ~31, first = min(n_pairs, (rank * 32 + warp) * per);
+    const int last = min(n_pairs, first + per);
     const int bits = 32 - __clz(E);
     for (int e = lane; e < E; e += 32) s_count[warp][e] = 0;
     __syncwarp();
-    for (int p0 = first; p0 < last; p0 += 32) {
-        const int p = p0 + lane, v = p < last ? idx[p] : E, e = v < 0 || v > E ? E : v;      // (E: none)
-        const unsigned same = moe_same(e, bits);
-        if (e < E && lane == __ffs(same) - 1) s_count[warp][e] += __popc(same);
-        __syncwarp();
+    constexpr int HELD = CTAS > 1 ? 8 : MOE_SORT_ONE / 1024;
+    int mine[HELD];                                          // the experts of 32 HELD pairs, loaded at once
+    auto load = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int p = base + 32 * i + lane, v = p < last ? idx[p] : E;
+            mine[i] = v < 0 || v > E ? E : v;                // (E: none)
+        }
+    };
+    for (int base = first; base < last; base += 32 * HELD) {
+        load(base);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            if (base + 32 * i >= last) break;
+            const int e = mine[i];
+            const unsigned same = moe_same(e, bits);
+            if (e < E && lane == __ffs(same) - 1) s_count[warp][e] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
-    if (tid < E) {                                           // what the warps before have of this expert, and all of it
+    int before = 0;                                          // what the blocks before have of expert `tid`
+    if (tid < E) {                                           // what the warps before have of it, and the block
         int run = 0;
 #pragma unroll
         for (int w = 0; w < 32; ++w) {
@@ -679,7 +703,27 @@ moe_sort_few_kernel(const int* idx, int n_pairs, int E, int* offsets, int* place
             s_count[w][tid] = run;
             run += c;
         }
-        s_first[tid] = run;
+        (CTAS > 1 ? s_block : s_first)[tid] = run;
+    }
+    if constexpr (CTAS > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (tid < E) {
+            int all = 0;
+#pragma unroll
+            for (int r = 0; r < CTAS; ++r) {
+                uint32_t at;
+                int c;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_block[tid])), "r"(r));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(at) : "memory");
+                all += c;
+                before += r < rank ? c : 0;
+            }
+            s_first[tid] = all;
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (this block has read the others' sums; waited for at the end)
     }
     __syncthreads();
     if (warp == 0) {                                         // exclusive prefix sum over the experts, 32 at a time
@@ -698,24 +742,36 @@ moe_sort_few_kernel(const int* idx, int n_pairs, int E, int* offsets, int* place
         if (lane == 0) s_first[E] = run;
     }
     __syncthreads();
-    for (int e = tid; e <= E; e += blockDim.x) offsets[e] = s_first[e];
-    for (int p0 = first; p0 < last; p0 += 32) {
-        const int p = p0 + lane, v = p < last ? idx[p] : E, e = v < 0 || v > E ? E : v;
-        const unsigned same = moe_same(e, bits);
-        const bool mine = e < E;
-        const int at = mine ? s_first[e] + s_count[warp][e] : 0;
-        __syncwarp();
-        if (mine) place[p] = at + __popc(same & ((1u << lane) - 1u));
-        if (mine && lane == __ffs(same) - 1) s_count[warp][e] += __popc(same);
-        __syncwarp();
+    if (tid <= E) {
+        if (rank == 0) offsets[tid] = s_first[tid];
+        s_first[tid] += before;
     }
+    __syncthreads();
+    for (int base = first; base < last; base += 32 * HELD) {
+        if (per > 32 * HELD) load(base);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            if (base + 32 * i >= last) break;
+            const int e = mine[i];
+            const unsigned same = moe_same(e, bits);
+            const int at = e < E ? s_first[e] + s_count[warp][e] : 0;
+            __syncwarp();
+            if (e < E) place[base + 32 * i + lane] = at + __popc(same & ((1u << lane) - 1u));
+            if (e < E && lane == __ffs(same) - 1) s_count[warp][e] += __popc(same);
+            __syncwarp();
+        }
+    }
+    if constexpr (CTAS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 RLLM_API int rllm_moe_sort(const int* idx, int* offsets, int* place, int n_pairs, int E, cudaStream_t stream) {
     if (n_pairs <= 0) return 0;
-    if (E <= 0 || E > MOE_MAX_EXPERTS) return (int)cudaErrorInvalidValue;
-    if (E <= MOE_SORT_E) return rllm_launch(moe_sort_few_kernel, dim3(1), dim3(1024), 0, stream, idx, n_pairs, E, offsets, place);
-    return rllm_launch(moe_sort_kernel, dim3((E + 31) / 32), dim3(1024), 0, stream, idx, n_pairs, E, offsets, place);
+    if (E <= 0 || E > MOE_MAX_EXPERTS || n_pairs > 0x7fff0000) return (int)cudaErrorInvalidValue;
+    if (E > MOE_SORT_E || n_pairs <= MOE_SORT_FEW)
+        return rllm_launch(moe_sort_kernel, dim3((E + 31) / 32), dim3(1024), 0, stream, idx, n_pairs, E, offsets, place);
+    if (n_pairs <= MOE_SORT_ONE)
+        return rllm_launch(moe_sort_few_kernel<1>, dim3(1), dim3(1024), 0, stream, idx, n_pairs, E, offsets, place);
+    return rllm_launch_clusters(moe_sort_few_kernel<8>, dim3(8), dim3(1024), 0, stream, dim3(8, 1, 1), idx, n_pairs, E, offsets, place);
 }
 
 // rows[place[pair]] = h[pair / top_k]: a block per token reads the row once (16 bytes a thread and turn where the

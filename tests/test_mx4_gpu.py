@@ -253,7 +253,8 @@ def test_experts_down(n, E, top, skew, F, d, many):
     ops().check_device_errors()
 
 
-@pytest.mark.parametrize("n,E,top", [(1, 1, 1), (3, 256, 2), (700, 16, 4), (1000, 255, 8), (2000, 256, 1), (900, 300, 3), (5000, 2, 2)])
+@pytest.mark.parametrize("n,E,top", [(1, 1, 1), (3, 256, 2), (700, 16, 4), (1000, 255, 8), (2000, 256, 1), (900, 300, 3), (5000, 2, 2),
+                                     (64, 33, 4), (257, 256, 1), (256, 1, 8), (683, 128, 3), (8192, 128, 8), (65537, 7, 1), (33000, 256, 5)])
 def test_sort_is_stable(n, E, top):
     """Pairs in the order of their experts, and within an expert in their own, with every number of experts a kernel takes."""
     idx = torch.randint(0, E, (n, top), generator=torch.Generator().manual_seed(n)).to(torch.int32).to(DEV)
