@@ -604,4 +604,6 @@ RLLM_API int rllm_mx4_product(const void* x, const int* offsets, const int* plac
                          glu_alpha, glu_shift, err, stream);
 }
 
+TC_DEFINE_WAIT_CONTROLS(rllm_gemm_mx4)
+
 RLLM_PACKED(rllm_mx4_product)
