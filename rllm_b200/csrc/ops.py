@@ -1475,6 +1475,14 @@ _error_words: dict = {}
 ERROR_CODES_RANGE = {4: "a token id outside the vocabulary", 5: "a cache slot outside the pool",
                      6: "a page outside the pool"}
 
+# what the kernels with bounded waits write when they give one up: the products (1 to 3), the prompt's attention (11 to 15), the grouped
+# products (21 to 23), those of 4-bit numbers for many (31 to 33) and for few rows (34 to 36)
+_WAIT_CODES = {at + i: what for at in (1, 21, 31, 34) for i, what in enumerate(
+    ("operand tiles never arrived", "a stage was never released", "the accumulator never completed"))}
+_WAIT_CODES.update({11: "the queries never arrived", 12: "a tile of keys or values, or what is multiplied with it, never came",
+                    13: "a tile's scores never completed", 14: "the product with a tile's values never completed",
+                    15: "a stage of keys or values was never released"})
+
 
 def error_word(device) -> torch.Tensor:
     """The device int into which kernels with bounded waits write a code when a wait runs out."""
@@ -1493,8 +1501,8 @@ def check_device_errors(device="cuda:0") -> None:
         if code in ERROR_CODES_RANGE:
             raise KernelError(f"a kernel refused an index (code {code}: {ERROR_CODES_RANGE[code]}); the access was "
                               f"skipped, the step's results are not to be used")
-        raise KernelError(f"a kernel's bounded wait ran out (code {code}: 1 operand tiles never arrived, "
-                          f"2 a stage was never released, 3 the accumulator never completed)")
+        what = _WAIT_CODES.get(code)
+        raise KernelError(f"a kernel's bounded wait ran out (code {code}{': ' + what if what else ''})")
 
 
 _WAIT_LIBRARIES = {"tc": "rllm_tc", "tc2": "rllm_tc2", "stream": "rllm_stream", "attn_tc": "rllm_attn_tc",
