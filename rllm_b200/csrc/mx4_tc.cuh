@@ -3,6 +3,7 @@
 #pragma once
 #include "tcgen05.cuh"
 #include "mx4.cuh"
+#include "asked_once.h"
 #include <math.h>
 
 #define MX4_SF_BYTES (2 * MX4_ATOM)                        // the scales of 128 rows in a stage of 256 entries along K
@@ -134,21 +135,12 @@ struct Mx4Glu {
 // ---------------------------------------------------------------- host side
 // Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the runtime once for each of them.
 template <typename F> static int mx4_allow_smem(F* kern, int bytes) {
-    static const void* seen[64];
-    static int seen_device[64], n_seen = 0;
+    static AskedOnce* const table = new AskedOnce;       // (never destroyed: threads may still launch while the process ends)
     int dev = 0;
     const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
-    for (int i = 0; i < n_seen; ++i)
-        if (seen[i] == (const void*)kern && seen_device[i] == dev) return 0;
-    const cudaError_t s = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (s != cudaSuccess) return (int)s;
-    if (n_seen < 64) {                                   // (two threads at once may each enter it, or lose an entry: asked again then)
-        seen[n_seen] = (const void*)kern;
-        seen_device[n_seen] = dev;
-        ++n_seen;
-    }
-    return 0;
+    return table->once((const void*)kern, dev,
+                       [&] { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
 }
 
 // Tensor map of codes [rows, k / 2] (contiguous): boxes of box_rows x 128 bytes, 128-byte swizzle, zeros outside.
