@@ -610,7 +610,8 @@ moe_sort_kernel(const int* __restrict__ idx, int n_pairs, int E, int* offsets, i
     __syncthreads();
     for (int p = tid; p < n_pairs; p += blockDim.x) {
         const int e = idx[p];
-        if (e >= 0 && e < E) atomicAdd(&s_count[e], 1);      // (a pair of no expert: no place)
+        if (e >= 0 && e < E) atomicAdd(&s_count[e], 1);
+        else if (blockIdx.x == 0) place[p] = -1;             // a pair of no expert: no place
     }
     __syncthreads();
     if (warp == 0) {                                       // exclusive prefix sum over the experts, 32 at a time
@@ -756,7 +757,8 @@ moe_sort_few_kernel(const int* idx, int n_pairs, int E, int* offsets, int* place
             const unsigned same = moe_same(e, bits);
             const int at = e < E ? s_first[e] + s_count[warp][e] : 0;
             __syncwarp();
-            if (e < E) place[base + 32 * i + lane] = at + __popc(same & ((1u << lane) - 1u));
+            const int p = base + 32 * i + lane;
+            if (p < last) place[p] = e < E ? at + __popc(same & ((1u << lane) - 1u)) : -1;
             if (e < E && lane == __ffs(same) - 1) s_count[warp][e] += __popc(same);
             __syncwarp();
         }
@@ -774,7 +776,7 @@ RLLM_API int rllm_moe_sort(const int* idx, int* offsets, int* place, int n_pairs
     return rllm_launch_clusters(moe_sort_few_kernel<8>, dim3(8), dim3(1024), 0, stream, dim3(8, 1, 1), idx, n_pairs, E, offsets, place);
 }
 
-// rows[place[pair]] = h[pair / top_k]: a block per token reads the row once (16 bytes a thread and turn where the
+// rows[place[pair]] = h[pair / top_k] (a pair without a place, -1, is left out): a block per token reads the row once (16 bytes a thread and turn where the
 // rows allow it) and writes it to the places of its top_k pairs
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -785,7 +787,7 @@ moe_gather_rows_kernel(const T* h, const int* __restrict__ place, T* rows, int t
     const int t = blockIdx.x;
     if (weight_out && (int)threadIdx.x < top_k) {
         const size_t p = (size_t)t * top_k + threadIdx.x;
-        weight_out[place[p]] = weight[p];
+        if (place[p] >= 0) weight_out[place[p]] = weight[p];
     }
     const T* src = h + (size_t)t * d;
     if (vec) {
@@ -793,14 +795,19 @@ moe_gather_rows_kernel(const T* h, const int* __restrict__ place, T* rows, int t
         const uint4* s4 = reinterpret_cast<const uint4*>(src);
         for (int i = threadIdx.x; i < n16; i += blockDim.x) {
             const uint4 u = s4[i];
-            for (int j = 0; j < top_k; ++j)
-                reinterpret_cast<uint4*>(rows + (size_t)place[(size_t)t * top_k + j] * d)[i] = u;
+            for (int j = 0; j < top_k; ++j) {
+                const int p = place[(size_t)t * top_k + j];
+                if (p >= 0) reinterpret_cast<uint4*>(rows + (size_t)p * d)[i] = u;
+            }
         }
         return;
     }
     for (int i = threadIdx.x; i < d; i += blockDim.x) {
         const T v = src[i];
-        for (int j = 0; j < top_k; ++j) rows[(size_t)place[(size_t)t * top_k + j] * d + i] = v;
+        for (int j = 0; j < top_k; ++j) {
+            const int p = place[(size_t)t * top_k + j];
+            if (p >= 0) rows[(size_t)p * d + i] = v;
+        }
     }
 }
 
@@ -818,7 +825,8 @@ RLLM_API int rllm_moe_gather_rows(const void* h, int dt, const int* place, void*
                        vec, weight, weight_out);
 }
 
-// out[t] = sum_j weight[t, j] * y[place[t * top_k + j]] (+ shared[t] * sigmoid(gate[t])); place null: y in pair order
+// out[t] = sum_j weight[t, j] * y[place[t * top_k + j]] (+ shared[t] * sigmoid(gate[t])); place null: y in pair order; pairs without a
+// place (-1) add nothing
 // A thread takes four neighbouring columns where the rows allow it (16-byte loads, a token's top_k rows in flight
 // side by side), one column otherwise; the columns of a token are spread over blockIdx.y.
 template <int VEC>
@@ -836,16 +844,19 @@ moe_combine_kernel(const float* y, const int* place, const float* weight, float*
     for (int v = 0; v < VEC; ++v) sum[v] = 0.f;
 #pragma unroll 4
     for (int j = 0; j < top_k; ++j) {
-        const float w = weight ? weight[(size_t)t * top_k + j] : 1.f;
-        const float* row = y + (size_t)(place ? place[(size_t)t * top_k + j] : t * top_k + j) * d + i;
+        const size_t pair = (size_t)t * top_k + j;
+        const long long at = place ? (long long)place[pair] : (long long)pair;
+        const float w = at < 0 ? 0.f : weight ? weight[pair] : 1.f;      // (a pair of no expert adds nothing)
+        const float* row = y + at * d + i;
         if constexpr (VEC == 4) {
-            const float4 r = *reinterpret_cast<const float4*>(row);
+            float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at >= 0) r = *reinterpret_cast<const float4*>(row);
             sum[0] += w * r.x;
             sum[1] += w * r.y;
             sum[2] += w * r.z;
             sum[3] += w * r.w;
         } else {
-            sum[0] += w * row[0];
+            sum[0] += w * (at < 0 ? 0.f : row[0]);
         }
     }
     if constexpr (VEC == 4) {

@@ -1243,7 +1243,8 @@ _moe_combine = _Packed("moe", "rllm_moe_combine", 6, 4)
 
 
 def moe_sort(idx, E):
-    """(offsets int32 [E + 1], place int32 [pairs]): the pairs of idx [n, top_k] in expert order (stable)."""
+    """(offsets int32 [E + 1], place int32 [pairs]): the pairs of idx [n, top_k] in expert order (stable).  A pair whose expert is none of
+    the E has no place (-1): gather, products and `moe_combine` leave it out."""
     _need_cuda(idx)
     _need_contig(idx=idx)
     offsets = torch.empty(E + 1, dtype=torch.int32, device=idx.device)
