@@ -1247,6 +1247,8 @@ def moe_sort(idx, E):
     the E has no place (-1): gather, products and `moe_combine` leave it out."""
     _need_cuda(idx)
     _need_contig(idx=idx)
+    if idx.numel() > 0x7fff0000:
+        raise KernelError(f"moe_sort: {idx.numel()} pairs, more than a launch counts")
     offsets = torch.empty(E + 1, dtype=torch.int32, device=idx.device)
     place = torch.empty(idx.numel(), dtype=torch.int32, device=idx.device)
     _check(_moe_sort((idx, offsets, place), (idx.numel(), E)), "moe_sort")
@@ -1990,6 +1992,7 @@ def gate_up_swiglu(h, w_gate_up, out, glu=None):
 
 MX4_BLOCK = 32                 # neighbouring entries of a row that share a scale
 MX4_MAX_EXPERTS = 1024
+MX4_MAX_ROWS = 0x7fffff00      # of a stack of matrices, or of rows (the kernels count them in 32 bits, and to the end of a tile)
 
 
 class Mx4Matrix:
@@ -2010,6 +2013,8 @@ class Mx4Matrix:
         k = 2 * half
         if k % MX4_BLOCK or k == 0:
             raise KernelError(f"Mx4Matrix: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
+        if codes.numel() > half * MX4_MAX_ROWS or k > MX4_MAX_ROWS:
+            raise KernelError(f"Mx4Matrix: {codes.numel() // half} rows of {k} entries, more than a launch counts")
         if scales.shape != (*lead, n + 127 >> 7, 2 * (k + 255 >> 8), 32, 4, 4) or scales.get_device() != codes.get_device():
             raise KernelError(f"Mx4Matrix: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous()) or (codes.data_ptr() | scales.data_ptr()) & 15:
@@ -2085,8 +2090,10 @@ def _mx4_rows(x, who):
     if x.dim() == 2:
         m, k = x.shape
         ld, one = x.stride()
-        if one == 1 and k and k % MX4_BLOCK == 0:
+        if one == 1 and k and k % MX4_BLOCK == 0 and m <= MX4_MAX_ROWS and k <= MX4_MAX_ROWS:
             return m, k, ld
+        if m > MX4_MAX_ROWS or k > MX4_MAX_ROWS:
+            raise KernelError(f"{who}: {m} rows of {k} entries, more than a launch counts")
         if k == 0 or k % MX4_BLOCK:
             raise KernelError(f"{who}: rows of {k} entries are not whole blocks of {MX4_BLOCK}")
     raise KernelError(f"{who}: rows [m, k] with neighbouring entries side by side, got {tuple(x.shape)} with strides {x.stride()}")

@@ -68,3 +68,23 @@ def test_plain_rounding():
     assert v[0, :12].tolist() == [0, 1, 1, 2, 2, 4, 4, 6, 0, -1, -4, 4]
     _, scales, v = plain.quantize((x * 2.0 ** -130)[None])
     assert scales.tolist() == [[0]] and v[0, 11] == 2.0 ** -128
+
+
+def test_refusal_of_sizes_beyond_31_bits(monkeypatch):
+    """The launchers take rows as 32-bit numbers: more of them would arrive as another number, or as none."""
+    monkeypatch.setattr(ops, "_mx4_current", lambda *t: None)               # (as on a GPU)
+    many = 1 << 31
+    x = torch.zeros(1, 64, dtype=torch.bfloat16).expand(many, 64)
+    w = ops.Mx4Matrix(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(ops.mx4_scale_shape(4, 64), dtype=torch.uint8))
+    out = torch.empty(many, 4, device="meta")
+    for call in (lambda: ops.mx4_quantize(x), lambda: ops.mx4_linear(x, w, out)):
+        with pytest.raises(ops.KernelError, match="2147483648 rows"):
+            call()
+    for lead, n in (((), many), ((2,), many // 2), ((1 << 20, 2), 1 << 10)):
+        codes = torch.empty(*lead, n, 32, dtype=torch.uint8, device="meta")
+        scales = torch.empty(*lead, *ops.mx4_scale_shape(n, 64), dtype=torch.uint8, device="meta")
+        with pytest.raises(ops.KernelError, match="2147483648 rows"):
+            ops.Mx4Matrix(codes, scales)
+    monkeypatch.setattr(ops, "_need_cuda", lambda *t: None)
+    with pytest.raises(ops.KernelError, match="2147483648 pairs"):
+        ops.moe_sort(torch.empty(many // 2, 2, dtype=torch.int32, device="meta"), 4)
