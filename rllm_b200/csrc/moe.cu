@@ -844,19 +844,20 @@ moe_combine_kernel(const float* y, const int* place, const float* weight, float*
     for (int v = 0; v < VEC; ++v) sum[v] = 0.f;
 #pragma unroll 4
     for (int j = 0; j < top_k; ++j) {
-        const size_t pair = (size_t)t * top_k + j;
-        const long long at = place ? (long long)place[pair] : (long long)pair;
-        const float w = at < 0 ? 0.f : weight ? weight[pair] : 1.f;      // (a pair of no expert adds nothing)
-        const float* row = y + at * d + i;
+        const float w = weight ? weight[(size_t)t * top_k + j] : 1.f;
+        const int at = place ? place[(size_t)t * top_k + j] : t * top_k + j;
+        const float* row = y + (size_t)max(at, 0) * d + i;   // (a pair of no expert adds nothing)
         if constexpr (VEC == 4) {
-            float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (at >= 0) r = *reinterpret_cast<const float4*>(row);
-            sum[0] += w * r.x;
-            sum[1] += w * r.y;
-            sum[2] += w * r.z;
-            sum[3] += w * r.w;
+            const float4 r = *reinterpret_cast<const float4*>(row);
+            if (at >= 0) {
+                sum[0] += w * r.x;
+                sum[1] += w * r.y;
+                sum[2] += w * r.z;
+                sum[3] += w * r.w;
+            }
         } else {
-            sum[0] += w * (at < 0 ? 0.f : row[0]);
+            const float r = row[0];
+            if (at >= 0) sum[0] += w * r;
         }
     }
     if constexpr (VEC == 4) {
