@@ -514,3 +514,27 @@ def test_few_rows_shared_k(m, bn, n, k, splits):
         o._mx4_product(x, g, act, (2,), o.EPI_SWIGLU, CLAMPED, "", few_gated)
         plain.near(act, *plain.gated(xq, gv[0], gv[1], CLAMPED))
     o.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_gated_far_below_zero(m, dtype, many):
+    """Gates whose sigmoid has a denominator between 2^126 and 2^128: small results, not zeros.  The products are sums of a few small whole
+    and half numbers, exact in any order; what may be off is e^88 by 2 + 1.173 * 88 ulp (of 2^-23), its argument with a factor by half a step of
+    88, and six more roundings and the division's 2 ulp: 2^-15 of the result covers them, with the output's half step."""
+    k, F = 64, 200
+    for form, x, w in ((None, (6, 6, 4, 0), (6, 6, 4, 0)), (CLAMPED, (6, 4, 6, 0.5), (6, 3, 0.5, 1))):
+        h = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV)
+        h[:, :4] = torch.tensor(x, dtype=torch.bfloat16)
+        up = torch.zeros(F, k, device=DEV)
+        up[:, :4] = torch.tensor(w, dtype=torch.float32)
+        up[5:] *= 0.5                                             # (the others' gates are moderate)
+        got = ops().gate_up_swiglu(h, ops().mx4_quantize(torch.stack([-up, up])), torch.empty(m, F, dtype=dtype, device=DEV), glu=form)
+        y = (h.double() @ up.double().T)
+        limit, alpha, shift = form or SWIGLU
+        alpha = float(torch.tensor(alpha, dtype=torch.float32))
+        gate, u = -y, y.clamp(max=limit) if limit else y
+        want = gate / (1 + torch.exp(-alpha * gate)) * (u + shift)
+        assert 87.4 < -alpha * float(gate[0, 0]) < 88.7
+        half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+        assert bool(((got.double() - want).abs() <= (2.0 ** -15 + half) * want.abs()).all()), (got[0, 0], want[0, 0])
