@@ -280,11 +280,8 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
         if (ep_ok) {
             tc_fence_after();
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + b_first;
-            if constexpr (COLS == 8) tmem_ld8(taddr, v);
-            else {
 #pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += 16) tmem_ld16(taddr + c0, v + c0);
-            }
+            for (int c0 = 0; c0 < COLS; c0 += 16) tmem_ld16(taddr + c0, v + c0);
             tmem_ld_wait();
         } else {
 #pragma unroll

@@ -93,11 +93,7 @@ __device__ __forceinline__ void warp_bulk_load(uint32_t on, uint32_t dst, const 
                  "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(s_addr(bar)), "r"(on) : "memory");
 }
-// 8 and 16 columns of the warp's lanes
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]) : "r"(taddr) : "memory");
-}
+// 16 columns of the warp's lanes
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
