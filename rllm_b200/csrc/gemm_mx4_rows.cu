@@ -1,14 +1,15 @@
 // Products of microscaled 4-bit numbers for few rows (decode): C[b, n] = sum_k Q(X)[b, k] W[n, k], rows X in bfloat16 or float32, W as
 // codes and scales (mx4.cuh).  What it cannot do without is reading W once, 17 bytes for 32 entries; so W is the streamed M side (128 rows
-// a CTA), 16, 32 or 64 rows of X are the N side, the columns of the accumulator, and
-//   * the rows become 4-bit numbers here: eight warps read the CTA's part of X, quantise it and write it into the stage that the
+// a CTA), 16, 32, 64 or 128 rows of X are the N side, the columns of the accumulator, and
+//   * the rows become 4-bit numbers here: four warps read the CTA's part of X, quantise it and write it into the stage that the
 //     product reads (the 128-byte swizzle and the scale atoms by hand), so that a product is one launch.  Every CTA repeats that for its part
 //     of K.  It is latency that counts: no division in the loop, loads up to eight rows ahead, several rows side by side.  That is for up to
 //     16 rows; more of them (TX uint8_t) come as codes and scales that a launch before has made, by the same copies as the weights;
 //   * weights that are settled start ahead of the dependency wait, as in the bfloat16 kernels;
 //   * a thread-block cluster of 2, 4 or 8 CTAs shares a tile's K where there are few tiles: partial sums are parked in shared memory, every
-//     CTA adds and writes its share of the tile's rows, in rank order, which is ascending k (no atomics, no global scratch).  The number of
-//     CTAs depends on W's shape alone, so a row's bits do not depend on the rows around it;
+//     CTA adds and writes its share of the tile's rows, in rank order, which is ascending k (no atomics, no global scratch).  With the same
+//     kernel and the same number of CTAs a row's bits do not depend on the rows around it.  But both follow from all the sizes, the number of
+//     rows among them (ops.mx4_few_rows, mx4_row_splits): from one number of rows to another its sums may differ in their last bits;
 //   * of a gated product the cluster's first half of CTAs takes 128 gate rows, the other half the 128 up rows of the same index.
 // Gated 8 x 2 x 12,288 x 4,096: 12.4 us (53.5 MB, 4.3 TB/s); 1 x 4,096 x 4,096: 6.3 us for 8.9 MB, a chain of latencies: rows in, quantised, product, sums
 // through the cluster, out; 1 x 151,936 x 4,096: 52 us (6.3 TB/s).

@@ -2243,7 +2243,9 @@ _SWIGLU = (0.0, 1.0, 0.0)
 def mx4_linear(x, w, out=None, out_dtype=None, accumulate=False):
     """out [m, n] (+)= Q(x) W^T: the rows x [m, k] (float32 or bfloat16) become 4-bit numbers as by `mx4_quantize`, w [n, k] is an
     Mx4Matrix; products of 4-bit numbers with float32 sums.  accumulate: `out` is float32 and the product is added to it (in L2, one addition an
-    element; sums below 2^-126 become zero)."""
+    element; sums below 2^-126 become zero).
+    Which kernel runs and how many CTAs share K follow from the sizes, the number of rows among them: a row's sums may differ in their last bits
+    from one number of rows to another, as they do between the kernels for bfloat16 weights; calls of one size give the same bits."""
     if out is None:
         if accumulate:
             raise KernelError("mx4_linear: accumulate needs an output to add to")

@@ -538,3 +538,29 @@ def test_gated_far_below_zero(m, dtype, many):
         assert 87.4 < -alpha * float(gate[0, 0]) < 88.7
         half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
         assert bool(((got.double() - want).abs() <= (2.0 ** -15 + half) * want.abs()).all()), (got[0, 0], want[0, 0])
+
+
+@pytest.mark.parametrize("m,bn,splits", [(8, 16, 8), (16, 16, 4), (13, 16, 1), (32, 32, 4), (33, 64, 4), (64, 64, 1), (128, 128, 4), (300, 128, 2), (300, 0, 1)])
+def test_a_row_alone_and_among_others(m, bn, splits, monkeypatch):
+    """With the same kernel and the same number of CTAs that share K a row's bits do not depend on the rows around it: the sizes decide the
+    order of the sums, and which rows stand where does not."""
+    o, n, k = ops(), 300, 4096
+    x = rnd(m, k, seed=1, dtype=torch.bfloat16) * torch.exp(2 * rnd(1, k, seed=4)).to(torch.bfloat16)
+    w, _ = weight(n, k, seed=2)
+    g, _ = weight(2, n, k, seed=3)
+    for pairs in (False, True) if not bn else (False,):          # (the gated product of 128 and more rows has no kernel for few)
+        monkeypatch.setattr(o, "mx4_pairs", lambda *a: pairs)
+        few, few_gated = (bn, splits) if bn else False, (bn, min(splits, 4)) if 0 < bn < 128 else False
+
+        def both(rows):
+            out, act = torch.empty(rows.shape[0], n, device=DEV), torch.empty(rows.shape[0], n, device=DEV)
+            o._mx4_product(rows, w, out, (), o.EPI_STORE, SWIGLU, "", few)
+            o._mx4_product(rows, g, act, (2,), o.EPI_SWIGLU, SWIGLU, "", few_gated)
+            return out, act
+        whole = both(x)
+        for r in (0, m // 2, m - 1):
+            assert all(torch.equal(a[0], b[r]) for a, b in zip(both(x[r:r + 1]), whole))
+        turn = torch.arange(m - 1, -1, -1, device=DEV)
+        assert all(torch.equal(a[turn], b) for a, b in zip(both(x[turn]), whole))
+        assert all(torch.equal(a, b) for a, b in zip(both(x), whole))
+    o.check_device_errors()
