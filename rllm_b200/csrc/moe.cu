@@ -17,7 +17,7 @@
 //                    that multiplies an expert's input is a factor of its first product's result, so it is applied
 //                    there, in float32 (null: none).
 //   moe_sort         pairs counted per expert, offsets, and each pair's place in expert order (a stable
-//                    counting sort by one block); moe_gather_rows copies the tokens' rows into that order
+//                    counting sort; -1 for a pair whose expert is none of them); moe_gather_rows copies the tokens' rows into that order
 //                    and moe_combine adds a token's expert outputs back in the order of j.
 #include "common.cuh"
 #include "activations.cuh"

@@ -2155,13 +2155,19 @@ def mx4_few_rows(rows: int, n: int, k: int, gated: bool, own: bool, experts: int
     bn 16 is one launch, but every CTA quantises its part of the rows again: up to 8 rows it is as fast as a launch ahead of it (gated
     8 x 12,288 x 4,096: 12.4 us against 13.6), beyond that with small matrices only (16 x 12,288 x 4,096 gated: 15.9 against 14.1; 16 x 4,096
     x 1,024: 4.9 against 4.3, where the second launch costs the host more than that).  Sorted rows: while experts have few each (of 16 experts of
-    768 x 2,048: 32 pairs 9.3 us against 13.5, 128 pairs 12.2 against 12.6, 256 pairs 14.2 against 12.9).
+    768 x 2,048: 32 pairs 9.3 us against 13.5, 128 pairs 12.2 against 12.6, 256 pairs 14.2 against 12.9)
+    and no more CTAs than that the SMs go through them seven times, fourteen times with six stages and more, beyond which their starts and ends cost more than the
+    other kernel's padded tiles (us, few / many; CTAs x stages: 256 experts of 2,048 x 512, 64 pairs 1,024 x 2 18.5 / 18.5, 128 pairs 2,048 x 2 34.6 / 22.6;
+    128 of 2,048 x 768, 64 pairs 1,024 x 3 14.5 / 15.6, 128 pairs 2,048 x 3 27.9 / 18.7; 64 of 2 x 1,536 x 1,024, 32 pairs 768 x 4 14.8 / 19.7, 128 pairs
+    1,536 x 4 30.7 / 27.6; 128 of 4,096 x 1,536, 64 pairs 2,048 x 6 34.9 / 40.0, 128 pairs 4,096 x 6 66.2 / 53.7; 256 of 2 x 512 x 2,048, 128 pairs
+    1,024 x 8 30.4 / 37.2, 256 pairs 2,048 x 8 56.4 / 49.3; 128 of 2 x 1,536 x 4,096, 64 pairs 1,536 x 16 60.7 / 63.1, 128 pairs 3,072 x 16 110 / 98; 64 of
+    2 x 2,048 x 4,096, 32 pairs 1,024 x 16 44.2 / 61.1, 64 pairs 2,048 x 16 76.8 / 69.6).
     bn 128 against tiles of 128 x 256, one an SM: as long as its CTAs all run at once, two an SM (512 x 4,096 x 4,096 12.0 us against 13.7,
     300 x 1,000 x 2,080 8.0 against 10.8, 1,024 x 6,144 x 4,096 21.7 against 22.0); not for gated products, where it takes twice the CTAs and
     exchanges their sums (100 x 1,536 x 2,048 9.3 against 8.5)."""
     tiles = -(-n // 128) * (2 if gated else 1)
     if experts:
-        if not own or rows > min(256, 8 * experts):
+        if not own or rows > min(256, 8 * experts) or tiles * min(experts, rows) > (14 if k > 5 * 256 else 7) * n_sm:
             return None
         return 16, mx4_row_splits(tiles * min(experts, rows), k, 16, gated, True, n_sm)
     if own and rows <= 16 and (rows <= 8 or tiles * k <= 1 << 16):

@@ -88,3 +88,14 @@ def test_refusal_of_sizes_beyond_31_bits(monkeypatch):
     monkeypatch.setattr(ops, "_need_cuda", lambda *t: None)
     with pytest.raises(ops.KernelError, match="2147483648 pairs"):
         ops.moe_sort(torch.empty(many // 2, 2, dtype=torch.int32, device="meta"), 4)
+
+
+def test_few_rows_of_many_experts():
+    """The product of few rows keeps to as many CTAs as the SMs go through a few times."""
+    for pairs, n, k, gated, experts, few in ((64, 2048, 512, False, 256, True), (128, 2048, 512, False, 256, False),
+                                             (128, 512, 2048, True, 256, True), (64, 4096, 1536, False, 128, True),
+                                             (128, 4096, 1536, False, 128, False), (32, 768, 2048, True, 16, True), (129, 768, 2048, True, 16, False)):
+        got = ops.mx4_few_rows(pairs, n, k, gated, True, experts)
+        assert (got is not None) == few, (pairs, n, k, gated, experts)
+        if few:
+            assert got[0] == 16 and -(-n // 128) * (2 if gated else 1) * min(experts, pairs) <= 14 * 148

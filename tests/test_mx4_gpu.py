@@ -564,3 +564,26 @@ def test_a_row_alone_and_among_others(m, bn, splits, monkeypatch):
         assert all(torch.equal(a[turn], b) for a, b in zip(both(x[turn]), whole))
         assert all(torch.equal(a, b) for a, b in zip(both(x), whole))
     o.check_device_errors()
+
+
+@pytest.mark.parametrize("n,top", [(4, 8), (16, 8), (64, 4)])
+def test_many_experts_with_few_rows_each(n, top):
+    """256 experts: few pairs through the kernel for few rows, more of them through the tiles for many, as the sizes lead."""
+    E, d, F = 256, 1024, 96
+    idx, _ = route(n, E, top, 0, seed=n)
+    offsets, place = ops().moe_sort(idx, E)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    used = idx.flatten().unique().tolist()
+    w_up, w_down = (ops().mx4_quantize(torch.randn(s, generator=g, device=DEV) * s[-1] ** -0.5) for s in ((E, 2, F, d), (E, d, F)))
+    h = rnd(n, d, seed=1, dtype=torch.bfloat16)
+    act = ops().mx4_experts_up(h, w_up, offsets, place, torch.empty(n * top, F, dtype=torch.bfloat16, device=DEV))
+    y = ops().mx4_experts_down(act, w_down, offsets, torch.empty(n * top, d, device=DEV))
+    up, down = w_up.dequantize(), w_down.dequantize()
+    hq, aq = plain.quantize(h)[2], plain.quantize(act)[2]
+    for e in used:
+        t, j = (idx == e).nonzero(as_tuple=True)
+        at = place.view(n, top)[t, j].long()
+        plain.near(act[at], *plain.gated(hq[t], up[e, 0].double(), up[e, 1].double(), SWIGLU), f"up {e}")
+        want, size = plain.product(aq[at], down[e].double())
+        plain.near(y[at], want, plain.product_slack(size, F), f"down {e}")
+    ops().check_device_errors()
