@@ -342,6 +342,7 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
                 write(b0, groups, n0 + row, sum);
             }
         }
+        __syncwarp();      // the lanes' rows of X may have ended at different turns
         // #2: nobody reads another CTA's shared memory any more
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
