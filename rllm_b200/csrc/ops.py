@@ -1256,7 +1256,7 @@ def moe_sort(idx, E):
 
 
 def moe_gather_rows(h, place, rows, top_k, weight=None, weight_out=None):
-    """rows[place[p]] = h[p // top_k] for every pair p, and weight_out[place[p]] = weight[p] if given."""
+    """rows[place[p]] = h[p // top_k] for every pair p that has a place (not -1), and weight_out[place[p]] = weight[p] if given."""
     _need_cuda(h, place, rows, weight, weight_out)
     _need_contig(h=h, place=place, rows=rows, weight=weight, weight_out=weight_out)
     assert weight_out is None or (weight.dtype == weight_out.dtype == torch.float32 and weight.numel() == weight_out.numel()
@@ -1297,7 +1297,7 @@ def gemm_group(a, w, out, offsets=None, row_scale=None, activation=None):
 
 def moe_combine(y, place, weight, out, shared=None, gate=None, top_k=None):
     """out[t] = sum_j weight[t, j] * y[place[t * top_k + j]] (+ shared[t] * sigmoid(gate[t])), float32;
-    place None: y holds the pairs in their own order.  weight None: every weight is 1 (`top_k` is then needed)."""
+    place None: y holds the pairs in their own order; pairs without a place (-1) add nothing.  weight None: every weight is 1 (`top_k` is then needed)."""
     _need_cuda(y, place, weight, out, shared, gate)
     _need_contig(y=y, place=place, weight=weight, out=out, shared=shared)
     n, d = out.shape
@@ -2281,7 +2281,7 @@ def _mx4_experts(experts, rows, offsets, place, who):
 def mx4_experts_up(h, w, offsets, place, act, glu=None):
     """The gated product of routed experts: act[place[p]] = glu(Q(h[p // top_k]) Wg[e]^T, Q(h[p // top_k]) Wu[e]^T) for the pairs p of
     h [n, d] with their experts e, sorted by `moe_sort` (offsets [E + 1], place [n * top_k]); w [E, 2, F, d] as an Mx4Matrix, act
-    [n * top_k, F].  Two launches, whatever the experts' counts; no host involvement."""
+    [n * top_k, F].  Two launches at most, whatever the experts' counts; no host involvement.  Pairs without a place (-1) are left out."""
     pairs, n = act.shape[0], h.shape[0]
     if len(w.shape) != 4:
         raise KernelError(f"mx4_experts_up: weights {w.shape} where [E, 2, F, d] is needed")
